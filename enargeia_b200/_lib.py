@@ -59,6 +59,10 @@ class AttnDecodeDims(C.Structure):
                                    "pad0", "pad1")]
 
 
+class PagesDims(C.Structure):
+    _fields_ = [(n, U32) for n in ("rows", "width", "pages", "page_tokens")]
+
+
 class ModelConfigC(C.Structure):
     _fields_ = [("layers", U32), ("hidden", U32), ("heads", U32), ("kv_heads", U32), ("head_dim", U32),
                 ("intermediate", U32), ("vocab", U32), ("rms_norm_eps", F32), ("rope_theta", F32)]
@@ -96,6 +100,12 @@ SIGNATURES = {
     "enx_cache_pack": (C.c_int32, [P, P, U32, U32, P]),
     "enx_silu_mul": (C.c_int32, [P, P, P, U32, P]),
     "enx_add": (C.c_int32, [P, P, P, U32, P]),
+    "enx_pages_workspace_bytes": (C.c_size_t, [U32, U32]),
+    "enx_pages_free": (C.c_int32, [P, P, P, P, P, U32, P, C.POINTER(PagesDims), P]),
+    "enx_pages_fork": (C.c_int32, [P, P, P, P, P, U32, P, C.POINTER(PagesDims), P]),
+    "enx_pages_grow": (C.c_int32, [P, P, P, P, P, U32, P, P, P, C.POINTER(PagesDims), P, P]),
+    "enx_pages_compact": (C.c_int32, [P, P, P, P, P, P, P, P, C.POINTER(PagesDims), P, P]),
+    "enx_pages_copy": (C.c_int32, [P, U32, U32, U32, P, U32, P, P, P]),
     "enx_create": (C.c_int32, [C.POINTER(ModelConfigC), C.c_int, C.POINTER(P)]),
     "enx_destroy": (C.c_int32, [P]),
     "enx_load_enargeia": (C.c_int32, [P, C.c_char_p]),

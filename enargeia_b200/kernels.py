@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import AttnDecodeDims, EmbeddingDims, MatmulQ4Dims, SampleDims, SamplingRow, call
+from ._lib import AttnDecodeDims, EmbeddingDims, MatmulQ4Dims, PagesDims, SampleDims, SamplingRow, call
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -139,6 +139,111 @@ def silu_mul(g, u, out, stream=None):
 def add(a, b, out, stream=None):
     call("enx_add", _ptr(a), _ptr(b), _ptr(out), a.numel(), _stream(stream))
     return out
+
+
+# ---- pages of a shared key/value cache -----------------------------------------------------------
+
+
+def _i32(t: torch.Tensor, *shape) -> C.c_void_p:
+    """Pointer of a contiguous int32 CUDA tensor, of this shape (None: any size there)."""
+    if t.dtype != torch.int32:
+        raise ValueError("expected an int32 tensor")
+    if len(shape) != t.dim() or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+        raise ValueError(f"expected an int32 tensor of shape {shape}, got {tuple(t.shape)}")
+    return _ptr(t)
+
+
+def _call_on(first: torch.Tensor, others, name: str, *args, stream=None) -> None:
+    """`call` with the stream appended, on the device that all the tensors have to be on."""
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"expected all tensors on {device}, got one on {t.device}")
+    if device.index == torch.cuda.current_device():
+        call(name, *args, _stream(stream))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _stream(stream))
+
+
+def _scratch(nbytes: int, like: torch.Tensor, stream=None) -> torch.Tensor:
+    """A workspace for one call: its memory is not handed out again before the call is done."""
+    if stream is None or like.device.index != torch.cuda.current_device():
+        with torch.cuda.device(like.device):
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    else:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    if stream is not None:
+        ws.record_stream(stream)
+    return ws
+
+
+def _enough(workspace: Optional[torch.Tensor], nbytes: int, like: torch.Tensor, stream) -> torch.Tensor:
+    if workspace is None:
+        return _scratch(nbytes, like, stream)
+    if workspace.numel() * workspace.element_size() < nbytes:
+        raise ValueError(f"the workspace has to have {nbytes} bytes")
+    return workspace
+
+
+def _pages_dims(table, lengths, refs, status, page_tokens):
+    rows, width = table.shape
+    return (_i32(table, None, None), _i32(lengths, rows), _i32(refs, None), _i32(status, 1),
+            PagesDims(rows, width, refs.numel(), page_tokens))
+
+
+def pages_free(table, lengths, refs, rows, keep, status, page_tokens, stream=None):
+    """Rows `rows` of the page table keep their first `keep` tokens; the pages behind lose a holder.
+
+    table int32 [rows, width], lengths int32 [rows], refs int32 [pages] (holders of each page) and
+    status int32 [1] (error bits of include/enx.h, added to) are the cache's state; lists are int32."""
+    t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
+    n = rows.numel()
+    _call_on(table, (lengths, refs, rows, keep, status), "enx_pages_free", t, l, r, _i32(rows, n), _i32(keep, n), n, st,
+             C.byref(d), stream=stream)
+
+
+def pages_fork(table, lengths, refs, src, dst, status, page_tokens, stream=None):
+    """Empty rows `dst` become further holders of the pages of rows `src`."""
+    t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
+    n = dst.numel()
+    _call_on(table, (lengths, refs, src, dst, status), "enx_pages_fork", t, l, r, _i32(src, n), _i32(dst, n), n, st,
+             C.byref(d), stream=stream)
+
+
+def pages_grow(table, lengths, refs, rows, add, pairs, count, status, page_tokens, workspace=None, stream=None):
+    """Room for `add` more tokens in rows `rows`; pairs int32 [n, 2] and count int32 [2] say which
+    pages to copy before they are written (`pages_copy`) and how many pages were taken."""
+    t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
+    n = rows.numel()
+    if pairs.shape[0] < n:
+        raise ValueError(f"pairs has to have {n} rows")
+    ws = _enough(workspace, _lib.load().enx_pages_workspace_bytes(d.rows, d.pages), table, stream)
+    _call_on(table, (lengths, refs, rows, add, pairs, count, status, ws), "enx_pages_grow", t, l, r, _i32(rows, n),
+             _i32(add, n), n, _i32(pairs, None, 2), _i32(count, 2), st, C.byref(d), _ptr(ws), stream=stream)
+
+
+def pages_compact(table, lengths, refs, table_out, refs_out, pairs, count, status, page_tokens, workspace=None,
+                  stream=None):
+    """Closes the used pages up to the front: the table and the counts under the new numbers, pairs
+    int32 [pages, 2] of pages to copy, count = (pairs, pages in use)."""
+    t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
+    if pairs.shape[0] < d.pages:
+        raise ValueError(f"pairs has to have {d.pages} rows")
+    ws = _enough(workspace, _lib.load().enx_pages_workspace_bytes(d.rows, d.pages), table, stream)
+    _call_on(table, (lengths, refs, table_out, refs_out, pairs, count, status, ws), "enx_pages_compact", t, l, r,
+             _i32(table_out, d.rows, d.width), _i32(refs_out, d.pages), _i32(pairs, None, 2), _i32(count, 2), st,
+             C.byref(d), _ptr(ws), stream=stream)
+
+
+def pages_copy(pool, pairs, count, status, stream=None):
+    """Copies page pairs[i, 0] onto page pairs[i, 1] in every layer of pool uint8 [layers, pages,
+    page bytes], for the first count[0] pairs."""
+    if pool.dtype != torch.uint8 or pool.dim() != 3:
+        raise ValueError("expected a uint8 pool [layers, pages, page bytes]")
+    layers, pages, nbytes = pool.shape
+    _call_on(pool, (pairs, count, status), "enx_pages_copy", _ptr(pool), layers, pages, nbytes, _i32(pairs, None, 2),
+             pairs.shape[0], _i32(count, None), _i32(status, 1), stream=stream)
 
 
 def to_device_u32(a) -> torch.Tensor:

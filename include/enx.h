@@ -223,6 +223,68 @@ ENX_API enx_status enx_silu_mul(const float* gate, const float* up, float* out, 
 ENX_API enx_status enx_add(const float* a, const float* b, float* out, uint32_t count, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Pages of a key/value cache shared by many sequences (no reference counterpart: its KVCache,
+ * src/runtime/kvcache.ts:47-154, is one contiguous range per session).
+ *
+ * Device arrays of the caller: table int32 [rows][width], the pages of each row's sequence in the
+ * order of its tokens; lengths int32 [rows], the tokens it holds; refs int32 [pages], how many
+ * rows hold each page (0: free).  Rows of length 0 hold nothing.  Lists of rows and numbers are
+ * device arrays too, so nothing here waits for the GPU and every call can be captured into a graph.
+ *
+ * A call does all of its list or nothing: where a row number is outside the table or listed twice,
+ * a number is negative or a row would outgrow its table, it raises ENX_PAGES_BAD_LIST in *status
+ * (device int32, bits are added, the caller clears them), and where pages run out
+ * ENX_PAGES_NONE_FREE, and changes nothing.  A page number outside the pool raises
+ * ENX_PAGES_BAD_PAGE and is passed over.  ENX_ERR_RANGE above 262144 rows, 2^28 pages or 2^31 - 1
+ * tokens a row. */
+typedef struct {
+    uint32_t rows, width, pages, page_tokens;
+} enx_pages_dims;
+
+#define ENX_PAGES_NONE_FREE 1
+#define ENX_PAGES_BAD_LIST 2
+#define ENX_PAGES_BAD_PAGE 4
+
+/* Scratch of enx_pages_grow and enx_pages_compact (8-byte aligned; calls that may overlap on the
+ * GPU, from other streams or in other graphs, need one each). */
+ENX_API size_t enx_pages_workspace_bytes(uint32_t rows, uint32_t pages);
+/* Row rows[i] keeps its first min(keep[i], length) tokens (0: none); a page behind them loses a
+ * holder and its table entry becomes -1. */
+ENX_API enx_status enx_pages_free(int32_t* table, int32_t* lengths, int32_t* refs, const int32_t* rows,
+                                  const int32_t* keep, uint32_t n, int32_t* status,
+                                  const enx_pages_dims* dims, void* stream);
+/* Row dst[i], which must be empty, becomes another holder of all of row src[i]'s pages.  A row may
+ * be the source of several; none is source and destination of one call. */
+ENX_API enx_status enx_pages_fork(int32_t* table, int32_t* lengths, int32_t* refs, const int32_t* src,
+                                  const int32_t* dst, uint32_t n, int32_t* status,
+                                  const enx_pages_dims* dims, void* stream);
+/* Room for add[i] more tokens in row rows[i], whose length grows by them: new pages are the lowest
+ * free ones in the order of the list.  A partly filled last page that other rows hold too is
+ * replaced by a new page, and pairs[j] = (old page, new page) asks for its bytes (enx_pages_copy);
+ * of rows that together are its only holders the first keeps it.  pairs int32 [n][2]; count
+ * int32 [2] = {pairs, pages taken}. */
+ENX_API enx_status enx_pages_grow(int32_t* table, int32_t* lengths, int32_t* refs, const int32_t* rows,
+                                  const int32_t* add, uint32_t n, int32_t* pairs, int32_t* count,
+                                  int32_t* status, const enx_pages_dims* dims, void* workspace,
+                                  void* stream);
+/* Closes the pages in use up to the front of the pool: with L of them, the i-th used page from page
+ * L on moves into the i-th free one below L.  Writes the table and the counts under the new
+ * numbers (table_out and refs_out may be table and refs), pairs[j] = (from, onto) for
+ * enx_pages_copy (int32 [pages][2]) and count = {pairs, L}.  Entries behind a row's length become
+ * -1. */
+ENX_API enx_status enx_pages_compact(const int32_t* table, const int32_t* lengths, const int32_t* refs,
+                                     int32_t* table_out, int32_t* refs_out, int32_t* pairs,
+                                     int32_t* count, int32_t* status, const enx_pages_dims* dims,
+                                     void* workspace, void* stream);
+/* Copies page pairs[i][0] onto page pairs[i][1] in every layer of pool [layers][pages][page_bytes]
+ * for the first min(count[0], capacity) pairs.  No page may be source and destination of one call,
+ * nor a destination twice (the calls above make no such pairs).  page_bytes a multiple of 16, the
+ * pool 16-byte aligned. */
+ENX_API enx_status enx_pages_copy(void* pool, uint32_t layers, uint32_t pages, uint32_t page_bytes,
+                                  const int32_t* pairs, uint32_t capacity, const int32_t* count,
+                                  int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Model context: WeightStore + KVCache + DecodeGraph + ForwardGraph + Session's step.
  * One context is used from one host thread and owns one CUDA stream.
  * ---------------------------------------------------------------------------------------- */

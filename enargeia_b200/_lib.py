@@ -63,6 +63,10 @@ class PagesDims(C.Structure):
     _fields_ = [(n, U32) for n in ("rows", "width", "pages", "page_tokens")]
 
 
+class Kv4Dims(C.Structure):
+    _fields_ = [(n, U32) for n in ("rows", "width", "pages", "page_tokens", "kv_heads", "head_dim", "dtype", "pad0")]
+
+
 class ModelConfigC(C.Structure):
     _fields_ = [("layers", U32), ("hidden", U32), ("heads", U32), ("kv_heads", U32), ("head_dim", U32),
                 ("intermediate", U32), ("vocab", U32), ("rms_norm_eps", F32), ("rope_theta", F32)]
@@ -106,6 +110,9 @@ SIGNATURES = {
     "enx_pages_grow": (C.c_int32, [P, P, P, P, P, U32, P, P, P, C.POINTER(PagesDims), P, P]),
     "enx_pages_compact": (C.c_int32, [P, P, P, P, P, P, P, P, C.POINTER(PagesDims), P, P]),
     "enx_pages_copy": (C.c_int32, [P, U32, U32, U32, P, U32, P, P, P]),
+    "enx_kv4_write": (C.c_int32, [P, P, C.POINTER(C.c_int64), U32, P, P, P, P, P, P, C.POINTER(Kv4Dims), P]),
+    "enx_attn_kv4": (C.c_int32, [P, C.POINTER(C.c_int64), P, P, P, P, P, U32, U32, U32, F32, C.POINTER(Kv4Dims), P, P]),
+    "enx_attn_kv4_workspace_bytes": (C.c_size_t, [U32, U32]),
     "enx_create": (C.c_int32, [C.POINTER(ModelConfigC), C.c_int, C.POINTER(P)]),
     "enx_destroy": (C.c_int32, [P]),
     "enx_load_enargeia": (C.c_int32, [P, C.c_char_p]),

@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import AttnDecodeDims, EmbeddingDims, MatmulQ4Dims, PagesDims, SampleDims, SamplingRow, call
+from ._lib import AttnDecodeDims, EmbeddingDims, Kv4Dims, MatmulQ4Dims, PagesDims, SampleDims, SamplingRow, call
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -144,45 +144,42 @@ def add(a, b, out, stream=None):
 # ---- pages of a shared key/value cache -----------------------------------------------------------
 
 
-def _i32(t: torch.Tensor, *shape) -> C.c_void_p:
-    """Pointer of a contiguous int32 CUDA tensor, of this shape (None: any size there)."""
-    if t.dtype != torch.int32:
-        raise ValueError("expected an int32 tensor")
-    if len(shape) != t.dim() or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+def _i32(t: torch.Tensor, *shape) -> int:
+    """Address of a contiguous int32 CUDA tensor, of this shape (None: any size there)."""
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
+        raise ValueError("expected a contiguous int32 CUDA tensor")
+    if t.shape != shape and (len(shape) != t.dim() or any(w is not None and w != g for w, g in zip(shape, t.shape))):
         raise ValueError(f"expected an int32 tensor of shape {shape}, got {tuple(t.shape)}")
-    return _ptr(t)
+    return t.data_ptr()
 
 
-def _call_on(first: torch.Tensor, others, name: str, *args, stream=None) -> None:
-    """`call` with the stream appended, on the device that all the tensors have to be on."""
-    device = first.device
-    for t in others:
-        if t is not None and t.device != device:
-            raise ValueError(f"expected all tensors on {device}, got one on {t.device}")
-    if device.index == torch.cuda.current_device():
-        call(name, *args, _stream(stream))
-    else:
-        with torch.cuda.device(device):
-            call(name, *args, _stream(stream))
+def _call_on(tensors, name: str, *args, stream=None) -> None:
+    """`call` with the stream appended, on the device that all the tensors (None: absent) are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"expected all tensors on one device, got {tensors[0].device} and {t.device}")
+    if index < 0:
+        raise ValueError("expected CUDA tensors")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return call(name, *args, _stream(stream))
+    call(name, *args, _raw_stream(index) if stream is None else stream.cuda_stream)
 
 
-def _scratch(nbytes: int, like: torch.Tensor, stream=None) -> torch.Tensor:
-    """A workspace for one call: its memory is not handed out again before the call is done."""
-    if stream is None or like.device.index != torch.cuda.current_device():
-        with torch.cuda.device(like.device):
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    else:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    if stream is not None:
-        ws.record_stream(stream)
-    return ws
+#: The current stream's handle without the Stream object around it (a few us less a call).
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _enough(workspace: Optional[torch.Tensor], nbytes: int, like: torch.Tensor, stream) -> torch.Tensor:
+    """The caller's workspace, or one for this call, whose memory is not handed out before it is done."""
     if workspace is None:
-        return _scratch(nbytes, like, stream)
-    if workspace.numel() * workspace.element_size() < nbytes:
-        raise ValueError(f"the workspace has to have {nbytes} bytes")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+        if stream is not None:
+            workspace.record_stream(stream)
+    elif workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous():
+        raise ValueError(f"the workspace has to have {nbytes} contiguous bytes")
     return workspace
 
 
@@ -199,7 +196,7 @@ def pages_free(table, lengths, refs, rows, keep, status, page_tokens, stream=Non
     status int32 [1] (error bits of include/enx.h, added to) are the cache's state; lists are int32."""
     t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
     n = rows.numel()
-    _call_on(table, (lengths, refs, rows, keep, status), "enx_pages_free", t, l, r, _i32(rows, n), _i32(keep, n), n, st,
+    _call_on((table, lengths, refs, rows, keep, status), "enx_pages_free", t, l, r, _i32(rows, n), _i32(keep, n), n, st,
              C.byref(d), stream=stream)
 
 
@@ -207,7 +204,7 @@ def pages_fork(table, lengths, refs, src, dst, status, page_tokens, stream=None)
     """Empty rows `dst` become further holders of the pages of rows `src`."""
     t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
     n = dst.numel()
-    _call_on(table, (lengths, refs, src, dst, status), "enx_pages_fork", t, l, r, _i32(src, n), _i32(dst, n), n, st,
+    _call_on((table, lengths, refs, src, dst, status), "enx_pages_fork", t, l, r, _i32(src, n), _i32(dst, n), n, st,
              C.byref(d), stream=stream)
 
 
@@ -219,7 +216,7 @@ def pages_grow(table, lengths, refs, rows, add, pairs, count, status, page_token
     if pairs.shape[0] < n:
         raise ValueError(f"pairs has to have {n} rows")
     ws = _enough(workspace, _lib.load().enx_pages_workspace_bytes(d.rows, d.pages), table, stream)
-    _call_on(table, (lengths, refs, rows, add, pairs, count, status, ws), "enx_pages_grow", t, l, r, _i32(rows, n),
+    _call_on((table, lengths, refs, rows, add, pairs, count, status, ws), "enx_pages_grow", t, l, r, _i32(rows, n),
              _i32(add, n), n, _i32(pairs, None, 2), _i32(count, 2), st, C.byref(d), _ptr(ws), stream=stream)
 
 
@@ -231,7 +228,7 @@ def pages_compact(table, lengths, refs, table_out, refs_out, pairs, count, statu
     if pairs.shape[0] < d.pages:
         raise ValueError(f"pairs has to have {d.pages} rows")
     ws = _enough(workspace, _lib.load().enx_pages_workspace_bytes(d.rows, d.pages), table, stream)
-    _call_on(table, (lengths, refs, table_out, refs_out, pairs, count, status, ws), "enx_pages_compact", t, l, r,
+    _call_on((table, lengths, refs, table_out, refs_out, pairs, count, status, ws), "enx_pages_compact", t, l, r,
              _i32(table_out, d.rows, d.width), _i32(refs_out, d.pages), _i32(pairs, None, 2), _i32(count, 2), st,
              C.byref(d), _ptr(ws), stream=stream)
 
@@ -242,8 +239,75 @@ def pages_copy(pool, pairs, count, status, stream=None):
     if pool.dtype != torch.uint8 or pool.dim() != 3:
         raise ValueError("expected a uint8 pool [layers, pages, page bytes]")
     layers, pages, nbytes = pool.shape
-    _call_on(pool, (pairs, count, status), "enx_pages_copy", _ptr(pool), layers, pages, nbytes, _i32(pairs, None, 2),
+    _call_on((pool, pairs, count, status), "enx_pages_copy", _ptr(pool), layers, pages, nbytes, _i32(pairs, None, 2),
              pairs.shape[0], _i32(count, None), _i32(status, 1), stream=stream)
+
+
+# ---- a paged cache held in 4 bits, and attention over it ---------------------------------------------
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _kv4_dims(pool, table, page_tokens, kv_heads, head_dim, dtype):
+    if dtype not in _DTYPES:
+        raise ValueError(f"expected float32, float16 or bfloat16, got {dtype}")
+    if pool.dtype != torch.uint8 or pool.dim() != 2:
+        raise ValueError("expected one layer's uint8 pool [pages, page bytes]")
+    if pool.shape[1] != kv4_page_bytes(page_tokens, kv_heads, head_dim):
+        raise ValueError(f"a page has {kv4_page_bytes(page_tokens, kv_heads, head_dim)} bytes, the pool's {pool.shape[1]}")
+    rows, width = table.shape
+    return Kv4Dims(rows, width, pool.shape[0], page_tokens, kv_heads, head_dim, _DTYPES[dtype], 0)
+
+
+def kv4_page_bytes(page_tokens: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of a page of the 4-bit cache (one layer): codes and parameters of K and V."""
+    return page_tokens * kv_heads * (head_dim + 8 * max(1, head_dim // 64))
+
+
+def _rows_of(t: torch.Tensor) -> int:
+    """Pointer of a CUDA tensor whose last axis is contiguous (its other strides go with the call)."""
+    if not t.is_cuda:
+        raise ValueError("expected a CUDA tensor")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError("the last axis has to be contiguous")
+    return t.data_ptr()
+
+
+def kv4_write(k, v, pool, table, seqs, positions, page_tokens, k_out=None, v_out=None, stream=None):
+    """Quantises k and v [tokens, kv_heads, head_dim] into the 4-bit cache: token i to position
+    positions[i] of table row seqs[i] (int32; a negative position is passed over).  k_out and v_out,
+    if given, receive the values that the cache now holds."""
+    tokens, kv_heads, hd = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError("k and v have to have one shape and type")
+    for o in (k_out, v_out):
+        if o is not None and (o.shape != k.shape or o.dtype != k.dtype):
+            raise ValueError("k_out and v_out have to have the shape and type of k")
+    d = _kv4_dims(pool, table, page_tokens, kv_heads, hd, k.dtype)
+    strides = (C.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    _call_on((k, v, pool, table, seqs, positions, k_out, v_out), "enx_kv4_write", _rows_of(k), _rows_of(v), strides, tokens,
+             _ptr(pool), _i32(table, None, None), _i32(seqs, tokens), _i32(positions, tokens), _ptr(k_out), _ptr(v_out),
+             C.byref(d), stream=stream)
+
+
+def attn_kv4(q, pool, table, lengths, out, kv_heads, page_tokens, seqs=None, scale=None, workspace=None, stream=None):
+    """Attention of each sequence's newest tokens over its 4-bit cache: q and out [batch, queries,
+    heads, head_dim] or [batch, heads, head_dim]; sequence b is table row seqs[b] (or b), and
+    lengths[row] counts its tokens, the queries' own included."""
+    if q.shape != out.shape or q.dtype != out.dtype:
+        raise ValueError("q and out have to have one shape and type")
+    if q.dim() == 3:
+        q = q.unsqueeze(1)
+    batch, queries, heads, hd = q.shape
+    d = _kv4_dims(pool, table, page_tokens, kv_heads, hd, q.dtype)
+    if lengths.shape != (d.rows,):
+        raise ValueError("lengths has to have an entry for each table row")
+    ws = _enough(workspace, _lib.load().enx_attn_kv4_workspace_bytes(batch, hd), q, stream)
+    strides = (C.c_int64 * 3)(q.stride(0), q.stride(1), q.stride(2))
+    _call_on((q, pool, table, lengths, out, seqs, ws), "enx_attn_kv4", _rows_of(q), strides, _ptr(pool),
+             _i32(table, None, None), _i32(lengths, None), None if seqs is None else _i32(seqs, batch), _ptr(out), batch,
+             queries, heads, hd ** -0.5 if scale is None else scale, C.byref(d), _ptr(ws), stream=stream)
+    return out
 
 
 def to_device_u32(a) -> torch.Tensor:

@@ -78,9 +78,9 @@ ENX_API enx_status enx_matmul_q4(const float* x, const uint32_t* packed, const f
  * serialise them.  Their bounded device waits record a sticky error word instead of hanging;
  * enx_raw_check reads it. */
 
-/* Report (then clear) the sticky error word of the raw tensor-core entry points:
- * ENX_ERR_TIMEOUT if a bounded wait gave up since the last check, whose outputs are then
- * invalid.  It first waits for ALL work on the current device (cudaDeviceSynchronize), including
+/* Report (then clear) the sticky error word of the raw tensor-core entry points and of
+ * enx_attn_kv4: ENX_ERR_TIMEOUT if a bounded wait gave up since the last check, whose outputs are
+ * then invalid.  It first waits for ALL work on the current device (cudaDeviceSynchronize), including
  * the streams of other enx contexts and of other libraries on that device, so it must not be
  * called while any stream of the device is being captured into a CUDA graph.  No reference
  * counterpart (WebGPU kernels have no device waits). */
@@ -283,6 +283,53 @@ ENX_API enx_status enx_pages_compact(const int32_t* table, const int32_t* length
 ENX_API enx_status enx_pages_copy(void* pool, uint32_t layers, uint32_t pages, uint32_t page_bytes,
                                   const int32_t* pairs, uint32_t capacity, const int32_t* count,
                                   int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * A paged key/value cache held in 4 bits (the reference's cache is f16 and contiguous:
+ * src/runtime/kvcache.ts:59-88, src/kernels/cache_variants.ts:81-414).
+ *
+ * One layer's pool is [pages][kv_heads][page_tokens * (head_dim + 8 * groups)] bytes, 16-byte
+ * aligned.  A kv head of a page is its K codes [page_tokens][head_dim / 2], its K parameters
+ * [page_tokens][groups] (f16 scale, f16 offset), then V the same way; a group is min(64, head_dim)
+ * neighbouring elements of a token's head, and code c stands for scale * c + offset, element 2i of
+ * a row in the low half of its byte i.  table and lengths are those of enx_pages_*.
+ * head_dim 32, 64 or 128; page_tokens 16, 32, 64 or 128. */
+#define ENX_F32 0
+#define ENX_F16 1
+#define ENX_BF16 2
+
+typedef struct {
+    uint32_t rows, width, pages, page_tokens; /* table int32 [rows][width] of page numbers */
+    uint32_t kv_heads, head_dim;
+    uint32_t dtype, pad0; /* type of k, v and their values, or of q and out */
+} enx_kv4_dims;
+
+/* Quantises tokens 0..tokens-1 of k and v (each [tokens][kv_heads][head_dim] with strides[0..3] =
+ * k's token and head strides, then v's, in elements) and writes token i to position positions[i] of
+ * table row seqs[i].  Per group: scale = f16((max - min) / 15), offset = f16(min), code =
+ * (x - offset) / scale to the nearest whole number (ties to even), 0 to 15; f16 saturates.  A
+ * group that holds a value which is not finite reads back as NaN.  Tokens with a negative position,
+ * or whose row, position or page is outside the table or the pool, are passed over.  k_out and v_out
+ * (contiguous, or NULL) receive the values that the cache now holds, so that a prompt's own attention
+ * can see what later tokens will.  No two tokens of a call may share a slot. */
+ENX_API enx_status enx_kv4_write(const void* k, const void* v, const int64_t* strides,
+                                 uint32_t tokens, uint8_t* pool, const int32_t* table,
+                                 const int32_t* seqs, const int32_t* positions, void* k_out,
+                                 void* v_out, const enx_kv4_dims* dims, void* stream);
+
+/* Attention of the `queries` newest tokens of each of `batch` sequences: sequence b is table row
+ * seqs[b] (seqs NULL: row b), its cache holds lengths[row] tokens, those of the queries included, and
+ * query j sees tokens 0 .. lengths[row] - queries + j.  q is [batch][queries][heads][head_dim] with
+ * strides[0..2] of its first three axes in elements, out the same, contiguous and 16-byte aligned;
+ * softmax of scale * q.k.  Query rows that see nothing are 0; where seqs[b] is no table row, out is left as it was (a
+ * padded batch); a page number outside the pool makes its sequence's rows NaN.  Softmax and sums in
+ * f32.  workspace: enx_attn_kv4_workspace_bytes, 16-byte aligned, one for each call that may overlap
+ * on the GPU.  enx_raw_check reports a bounded wait that gave up. */
+ENX_API enx_status enx_attn_kv4(const void* q, const int64_t* strides, const uint8_t* pool,
+                                const int32_t* table, const int32_t* lengths, const int32_t* seqs,
+                                void* out, uint32_t batch, uint32_t queries, uint32_t heads,
+                                float scale, const enx_kv4_dims* dims, void* workspace, void* stream);
+ENX_API size_t enx_attn_kv4_workspace_bytes(uint32_t batch, uint32_t head_dim);
 
 /* ------------------------------------------------------------------------------------------
  * Model context: WeightStore + KVCache + DecodeGraph + ForwardGraph + Session's step.

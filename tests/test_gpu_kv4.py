@@ -1,0 +1,340 @@
+"""The paged 4-bit cache (enx_kv4_write, enx_attn_kv4) against its host twin in 64 bits.
+
+What the cache holds is compared bit for bit.  Attention's bound is that of the twin (f32 sums); for
+16-bit rows each weight is rounded to f16 too (2^-11), and every output to its type (half a step)."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kv4_twin as twin
+from enargeia_b200 import kernels as K
+from enargeia_b200._lib import EnxError
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def i32(v):
+    return torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")
+
+
+def rows(rng, shape, dtype):
+    x = rng.standard_normal(shape) + 1.5 * rng.standard_normal(shape[-2:])
+    return torch.from_numpy(x.astype(np.float32)).to(dtype).cuda()
+
+
+def tables(rng, lengths, page, spare=2, width=None):
+    need = [-(-n // page) for n in lengths]
+    order = rng.permutation(sum(need) + spare)
+    t = np.full((len(lengths), width or max(1, max(need))), -1, np.int64)
+    at = 0
+    for r, n in enumerate(need):
+        t[r, :n] = order[at:at + n]
+        at += n
+    return t, sum(need) + spare
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("kv,hd,page", [(2, 64, 16), (2, 32, 64), (1, 128, 32), (3, 128, 128), (5, 64, 128)])
+def test_write_is_the_twin_bit_for_bit(gpu, dtype, kv, hd, page):
+    rng = np.random.default_rng(kv * hd + page)
+    lengths = [1, 37, 2 * page, 3]
+    table, pages = tables(rng, lengths, page)
+    k, v = rows(rng, (sum(lengths), kv, hd), dtype), rows(rng, (sum(lengths), kv, hd), dtype)
+    k[0] = 0.25  # a group of one value
+    k[1, 0, :] = torch.arange(hd, device="cuda").to(dtype) % 16  # codes on the borders and exactly on the grid
+    k[2, 0, :] = torch.arange(hd, device="cuda").to(dtype) % 31 / 2
+    v[1] *= 1e-7  # scales below the normal f16 numbers
+    v[3] *= 1e4 if dtype == F16 else 1e7  # and above them
+    v[4, 0, 5], k[5, 0, 3] = math.nan, math.inf
+    seqs = np.repeat(np.arange(4), lengths)
+    positions = np.concatenate([np.arange(n) for n in lengths])
+    order = rng.permutation(len(seqs))  # tokens in any order
+    pool = torch.full((pages, K.kv4_page_bytes(page, kv, hd)), 0xAB, dtype=torch.uint8, device="cuda")
+    ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+    K.kv4_write(k, v, pool, i32(table), i32(seqs[order]), i32(positions[order]), page, ko, vo)
+    want = twin.Pool(pages, page, kv, hd, 0xAB)
+    for which, (x, back) in enumerate(((k, ko), (v, vo))):
+        c, s, o = twin.quantise(x.float().cpu().numpy())
+        for i, j in enumerate(order):
+            want.put(table[seqs[j], positions[j] // page], positions[j] % page, which, c[i], s[i], o[i])
+        held = torch.from_numpy(twin.values(c, s, o).astype(np.float32)).to(dtype)
+        assert torch.equal(back.cpu().nan_to_num(7.0, 8.0, 9.0), held.nan_to_num(7.0, 8.0, 9.0))
+    got = pool.cpu().numpy()
+    nan = 0x7E  # any NaN pattern is one: both sides use the quiet one
+    assert (got == want.bytes).all(), nan
+
+
+def test_write_strides_and_passed_over_tokens(gpu):
+    rng = np.random.default_rng(9)
+    kv, hd, page = 2, 64, 32
+    wide = rows(rng, (12, 3 * kv + 1, hd + 1), F16)
+    k, v = wide[:, 1:1 + kv, 1:], wide[:, 3:3 + 2 * kv:2, :hd]  # odd starts and strides
+    table = i32([[1, 99], [2, -1]])
+    seqs = i32([0, 1, 2, -1, 0, 0, 0, 1, 1, 0, 1, 1])
+    positions = i32([0, 5, 1, 1, -1, 64, 33, 33, 6, 31, 0, 31])
+    good = [0, 1, 8, 9, 10, 11]  # rows, positions and pages that exist
+    pool = torch.zeros(3, K.kv4_page_bytes(page, kv, hd), dtype=torch.uint8, device="cuda")
+    ko, vo = torch.full((12, kv, hd), 3.0, dtype=F16, device="cuda"), torch.full((12, kv, hd), 4.0, dtype=F16, device="cuda")
+    K.kv4_write(k, v, pool, table, seqs, positions, page, ko, vo)
+    want = twin.Pool(3, page, kv, hd)
+    for i in good:
+        for which, x in enumerate((k, v)):
+            want.put(int(table[seqs[i], positions[i] // page]), int(positions[i]) % page, which,
+                     *twin.quantise(x[i].float().cpu().numpy()))
+    assert (pool.cpu().numpy() == want.bytes).all()
+    skipped = [i for i in range(12) if i not in good]
+    assert (ko[skipped] == 3).all() and (vo[skipped] == 4).all()
+    K.kv4_write(k[:0], v[:0], pool, table, seqs[:0], positions[:0], page)
+
+
+def cache(rng, lengths, kv, hd, page, spare=2, width=None):
+    """A twin pool whose unused bytes are NaN parameters, its table, and K and V per sequence."""
+    table, pages = tables(rng, lengths, page, spare, width)
+    pool = twin.Pool(pages, page, kv, hd, 0xFF)
+    ks, vs = [], []
+    for r, n in enumerate(lengths):
+        for which, kept in ((0, ks), (1, vs)):
+            x = (rng.standard_normal((n, kv, hd)) + rng.standard_normal((kv, hd))).astype(np.float32)
+            c, s, o = twin.quantise(x)
+            for i in range(n):
+                pool.put(table[r, i // page], i % page, which, c[i], s[i], o[i])
+            kept.append((twin.values(c, s, o), twin.magnitudes(c, s, o)))
+    return table, pool, ks, vs
+
+
+def check(q, out, lengths, ks, vs, scale, order=None):
+    queries = q.shape[1]
+    half = torch.finfo(out.dtype).eps / 2
+    for b in range(q.shape[0]):
+        r = b if order is None else order[b]
+        want, bound = twin.attention(q[b].double().cpu().numpy(), ks[r][0], vs[r][0], scale, queries, ks[r][1], vs[r][1],
+                                     0.0 if out.dtype == F32 else 2.0 ** -11)
+        got = out[b].double().cpu().numpy()
+        off = np.abs(got - want) - (bound * (1 + half) + half * np.abs(want))
+        assert np.isfinite(got).all() and (off <= 1e-30).all(), (b, float(off.max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,kv,hd,page,queries", [(14, 2, 64, 16, 1), (4, 2, 32, 32, 1), (4, 1, 128, 64, 1),
+                                                      (16, 1, 128, 128, 1), (3, 3, 64, 32, 1), (14, 2, 64, 64, 4),
+                                                      (6, 2, 32, 16, 7), (10, 2, 128, 16, 3), (9, 1, 64, 128, 2)])
+def test_attention(gpu, heads, kv, hd, page, queries, dtype):
+    rng = np.random.default_rng(heads * hd + page)
+    lengths = [0, 1, 2, 15, 16, 17, 127, 128, 129, 300, 513]
+    table, pool, ks, vs = cache(rng, lengths, kv, hd, page)
+    q = torch.from_numpy(rng.standard_normal((len(lengths), queries, heads, hd)).astype(np.float32)).to(dtype).cuda()
+    out = torch.full_like(q, 7.0)
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32(lengths), out, kv, page)
+    check(q, out, lengths, ks, vs, hd ** -0.5)
+
+
+def test_one_long_sequence_is_shared_by_many_blocks(gpu):
+    rng = np.random.default_rng(3)
+    lengths = [9000, 5, 4097]
+    table, pool, ks, vs = cache(rng, lengths, 1, 64, 64)
+    q = torch.from_numpy(rng.standard_normal((3, 1, 5, 64)).astype(np.float32)).cuda()
+    outs = []
+    for _ in range(3):
+        out = torch.full_like(q, 7.0)
+        K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32(lengths), out, 1, 64)
+        outs.append(out)
+    check(q, outs[0], lengths, ks, vs, 0.125)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_rising_scores_and_wild_scales(gpu, dtype):
+    """Scores that climb along the sequence move the softmax's reference many times; V's scales span
+    the f16 range; one row dominates."""
+    rng = np.random.default_rng(4)
+    n, hd, page = 700, 64, 16
+    table, pool, ks, vs = cache(rng, [n], 1, hd, page)
+    k = (rng.standard_normal((n, 1, hd)) * 0.1 + np.linspace(-3, 3, n)[:, None, None]).astype(np.float32)
+    v = (rng.standard_normal((n, 1, hd)) * 10.0 ** rng.uniform(-5, 3, (n, 1, 1))).astype(np.float32)
+    for which, x, kept in ((0, k, ks), (1, v, vs)):
+        c, s, o = twin.quantise(x)
+        for i in range(n):
+            pool.put(table[0, i // page], i % page, which, c[i], s[i], o[i])
+        kept[0] = (twin.values(c, s, o), twin.magnitudes(c, s, o))
+    q = torch.from_numpy(np.abs(rng.standard_normal((1, 1, 6, hd))).astype(np.float32)).to(dtype).cuda()
+    q[0, 0, 1] *= -1
+    q[0, 0, 2] = 0
+    q[0, 0, 3] *= 1e-3
+    q[0, 0, 4, 1:] = 0
+    out = torch.empty_like(q)
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32([n]), out, 1, page, scale=0.3)
+    check(q, out, [n], ks, vs, 0.3)
+
+
+def test_padded_batch_strides_and_three_axes(gpu):
+    rng = np.random.default_rng(5)
+    lengths = [40, 0, 200]
+    table, pool, ks, vs = cache(rng, lengths, 2, 64, 32, width=9)
+    order = [2, -1, 0, 1, 3, 2]  # a row twice, none, one outside the table
+    wide = torch.from_numpy(rng.standard_normal((6, 20, 65)).astype(np.float32)).cuda()
+    q = wide[:, 3:17, 1:]
+    out = torch.full((6, 14, 64), 7.0, device="cuda")
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32(lengths), out, 2, 32, seqs=i32(order))
+    assert (out[1] == 7).all() and (out[4] == 7).all() and (out[3] == 0).all()
+    for b in (0, 2, 5):
+        check(q[b:b + 1, None], out[b:b + 1, None], lengths, ks, vs, 0.125, [order[b]])
+
+
+def test_pages_outside_the_pool_poison_their_sequence(gpu):
+    rng = np.random.default_rng(6)
+    table, pool, ks, vs = cache(rng, [50, 50, 50], 1, 64, 16)
+    table[0, 3], table[2, 0] = pool.bytes.shape[0], -1
+    q = torch.from_numpy(rng.standard_normal((3, 1, 2, 64)).astype(np.float32)).cuda()
+    out = torch.zeros_like(q)
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32([50, 50, 50]), out, 1, 16)
+    assert out[0].isnan().all() and out[2].isnan().all()
+    check(q[1:2], out[1:2], [50], ks[1:2], vs[1:2], 0.125)
+    # lengths outside the table are cut to it
+    out.zero_()
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32([-3, 1 << 30, 50]), out, 1, 16)
+    assert (out[0] == 0).all()
+
+
+def test_a_page_whose_values_are_not_finite(gpu):
+    """NaN in a token that a query does not see leaves it alone, and reaches those that see it."""
+    rng = np.random.default_rng(7)
+    table, pool, ks, vs = cache(rng, [20], 1, 64, 16)
+    bad = np.full((1, 64), np.nan, np.float32)
+    pool.put(table[0, 19 // 16], 19 % 16, 1, *twin.quantise(bad))
+    q = torch.from_numpy(rng.standard_normal((1, 2, 2, 64)).astype(np.float32)).cuda()
+    out = torch.zeros_like(q)
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32([20]), out, 1, 16)
+    assert out[0, 1].isnan().all()
+    # (the twin's weights of unseen tokens are absent, not zero)
+    want, bound = twin.attention(q[0].double().cpu().numpy(), ks[0][0], vs[0][0], 0.125, 2, ks[0][1], vs[0][1])
+    assert (np.abs(out[0, 0].cpu().numpy() - want[0]) <= bound[0] + 2.0 ** -24 * np.abs(want[0])).all()
+
+
+def test_write_grow_attend_in_one_captured_step(gpu):
+    """A decode step as a server runs it: room for a token, its write and the attention over it,
+    captured once and replayed, with rows forked from one prompt."""
+    rng = np.random.default_rng(8)
+    heads, kv, hd, page, n = 4, 2, 32, 16, 21
+    table, lengths = i32(np.full((3, 4), -1)), i32([0, 0, 0])
+    refs, status, count = i32([0] * 12), i32([0]), i32([0, 0])
+    pool = torch.full((1, 12, K.kv4_page_bytes(page, kv, hd)), 0xFF, dtype=torch.uint8, device="cuda")
+    pairs = i32([[0, 0]] * 3)
+    prompt_k, prompt_v = rows(rng, (n, kv, hd), F32), rows(rng, (n, kv, hd), F32)
+    K.pages_grow(table, lengths, refs, i32([0]), i32([n]), pairs, count, status, page)
+    K.kv4_write(prompt_k, prompt_v, pool[0], table, i32([0] * n), i32(np.arange(n)), page)
+    K.pages_fork(table, lengths, refs, i32([0, 0]), i32([1, 2]), status, page)
+    every, one = i32([0, 1, 2]), i32([1, 1, 1])
+    step_k, step_v = torch.zeros(3, kv, hd, device="cuda"), torch.zeros(3, kv, hd, device="cuda")
+    q, out = torch.zeros(3, heads, hd, device="cuda"), torch.zeros(3, heads, hd, device="cuda")
+    ws = torch.empty(K._lib.load().enx_attn_kv4_workspace_bytes(3, hd), dtype=torch.uint8, device="cuda")
+    ps = torch.empty(K._lib.load().enx_pages_workspace_bytes(3, 12), dtype=torch.uint8, device="cuda")
+
+    def step():
+        at = lengths.clone()
+        K.pages_grow(table, lengths, refs, every, one, pairs, count, status, page, ps)
+        K.pages_copy(pool, pairs, count, status)
+        K.kv4_write(step_k, step_v, pool[0], table, every, at, page)
+        K.attn_kv4(q, pool[0], table, lengths, out, kv, page, workspace=ws)
+
+    saved = [x.clone() for x in (table, lengths, refs, pool)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for x, y in zip((table, lengths, refs, pool), saved):
+        x.copy_(y)
+
+    def held(x):
+        c = twin.quantise(x.cpu().numpy())
+        return np.stack([twin.values(*c), twin.magnitudes(*c)])
+
+    k, v = [held(prompt_k)] * 3, [held(prompt_v)] * 3
+    for turn in range(14):
+        for x in (step_k, step_v, q):
+            x.copy_(torch.from_numpy(rng.standard_normal(x.shape).astype(np.float32)))
+        graph.replay()
+        k = [np.concatenate([k[b], held(step_k[b:b + 1])], 1) for b in range(3)]
+        v = [np.concatenate([v[b], held(step_v[b:b + 1])], 1) for b in range(3)]
+        check(q[:, None], out[:, None], None, k, v, hd ** -0.5)
+    assert status.item() == 0 and lengths.tolist() == [35, 35, 35] and sorted(refs.tolist()) == [0] * 5 + [1] * 6 + [3]
+    K.raw_check()
+
+
+def test_another_stream(gpu):
+    rng = np.random.default_rng(11)
+    table, pool, ks, vs = cache(rng, [400, 90], 1, 64, 64)
+    q = torch.from_numpy(rng.standard_normal((2, 1, 4, 64)).astype(np.float32)).cuda()
+    dev, out, t, n = torch.from_numpy(pool.bytes).cuda(), torch.zeros_like(q), i32(table), i32([400, 90])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    K.attn_kv4(q, dev, t, n, out, 1, 64, stream=side)
+    side.synchronize()
+    check(q, out, [400, 90], ks, vs, 0.125)
+
+
+def test_a_cache_behind_32_bits(gpu):
+    pages, kv, hd, page = 30000, 8, 128, 128
+    pool = torch.empty(pages, K.kv4_page_bytes(page, kv, hd), dtype=torch.uint8, device="cuda")  # 4.4 GB
+    rng = np.random.default_rng(12)
+    n = 130
+    k, v = rows(rng, (n, kv, hd), BF16), rows(rng, (n, kv, hd), BF16)
+    table = i32([[pages - 1, pages - 2]])
+    K.kv4_write(k, v, pool, table, i32([0] * n), i32(np.arange(n)), page)
+    q = rows(rng, (1, 1, 16, hd), BF16)
+    out = torch.zeros_like(q)
+    K.attn_kv4(q, pool, table, i32([n]), out, kv, page)
+    held = []
+    for x in (k, v):
+        c, s, o = twin.quantise(x.float().cpu().numpy())
+        held.append((twin.values(c, s, o), twin.magnitudes(c, s, o)))
+    check(q, out, [n], held[:1], held[1:], hd ** -0.5)
+
+
+def test_a_wait_that_gives_up_is_reported(gpu):
+    rng = np.random.default_rng(13)
+    table, pool, ks, vs = cache(rng, [600], 1, 64, 64)
+    q = torch.from_numpy(rng.standard_normal((1, 1, 4, 64)).astype(np.float32)).cuda()
+    dev, out, t, n = torch.from_numpy(pool.bytes).cuda(), torch.zeros_like(q), i32(table), i32([600])
+    K.raw_check()
+    try:
+        K.set_wait_limit(1)  # one poll, which may be enough or not
+        K.attn_kv4(q, dev, t, n, out, 1, 64)
+        try:
+            K.raw_check()
+            check(q, out, [600], ks, vs, 0.125)
+        except EnxError as e:
+            assert e.status == 5
+    finally:
+        K.set_wait_limit(0)
+    K.attn_kv4(q, dev, t, n, out, 1, 64)
+    K.raw_check()
+    check(q, out, [600], ks, vs, 0.125)
+
+
+def test_refused_arguments(gpu):
+    q = torch.zeros(2, 1, 4, 64, device="cuda")
+    pool = torch.zeros(3, K.kv4_page_bytes(16, 2, 64), dtype=torch.uint8, device="cuda")
+    t, n = i32([[0], [1]]), i32([1, 1])
+    ok = dict(q=q, pool=pool, table=t, lengths=n, out=torch.zeros_like(q), kv_heads=2, page_tokens=16)
+    K.attn_kv4(**ok)
+    for bad in (dict(q=q.double(), out=q.double()), dict(out=torch.zeros_like(q).half()), dict(pool=pool[:, :-16].contiguous()),
+                dict(table=t.long()), dict(lengths=i32([1])), dict(seqs=i32([0])), dict(page_tokens=8), dict(kv_heads=3),
+                dict(scale=0.0), dict(scale=math.nan), dict(workspace=torch.empty(16, dtype=torch.uint8, device="cuda")),
+                dict(q=q.transpose(2, 3).contiguous().transpose(2, 3)), dict(q=q.cpu()), dict(table=t[:1])):
+        with pytest.raises((ValueError, EnxError)):
+            K.attn_kv4(**{**ok, **bad})
+    k = torch.zeros(2, 2, 64, device="cuda")
+    good = dict(k=k, v=k, pool=pool, table=t, seqs=n, positions=n, page_tokens=16)
+    for bad in (dict(v=k.half()), dict(seqs=n[:1]), dict(positions=n.float()), dict(k_out=k.half()), dict(v_out=k[:1]),
+                dict(k=k[:, :, :63], v=k[:, :, :63]), dict(pool=pool[None]), dict(k_out=torch.zeros(2, 64, 2, device="cuda").mT)):
+        with pytest.raises((ValueError, EnxError)):
+            K.kv4_write(**{**good, **bad})

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) k_kv4_write(WriteArgs a) {
         const T* src = static_cast<const T*>(kv ? a.v : a.k) + (long long)token * (kv ? a.v_token : a.k_token) +
                        (long long)head * (kv ? a.v_head : a.k_head) + e8 * 8;
         if (a.vec) {
-            T tmp[8];
+            alignas(16) T tmp[8];
 #pragma unroll
             for (uint32_t i = 0; i < sizeof(T) / 2; ++i)
                 reinterpret_cast<uint4*>(tmp)[i] = ld_stream(reinterpret_cast<const uint4*>(src) + i);
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(256) k_kv4_write(WriteArgs a) {
     void* back = kv ? a.v_out : a.k_out;
     if (back) {
         T* dst = static_cast<T*>(back) + ((size_t)token * a.kv_heads + head) * a.hd + e8 * 8;
-        T tmp[8];
+        alignas(16) T tmp[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) tmp[i] = from_f<T>(val[i]);
         if (a.vec) {
@@ -171,6 +171,7 @@ struct AttnArgs {
     float* part;                            // partials: [2 * runs][8 NT][hd + 4]: sums, then m, l
     uint32_t batch, queries, heads, kv_heads, rows, width, pages, page_shift, tiles, most_chunks;
     float scale_log2;  // the softmax scale times log2(e)
+    int vec;           // q's rows start on 16 bytes
 };
 
 __device__ __forceinline__ uint32_t su32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -248,6 +249,8 @@ struct Cursor {
     int32_t row;
 };
 
+__device__ __forceinline__ uint32_t kv_head_of(const AttnArgs& a, uint32_t part) { return a.tiles == 1 ? part : part / a.tiles; }
+
 __device__ __forceinline__ uint32_t chunks_of(uint32_t len) { return (len + kKvChunk - 1) / kKvChunk; }
 
 // Table row and length of batch entry b; row -1: not to be computed.
@@ -276,7 +279,7 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
         reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
         reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-        T h[8];
+        alignas(16) T h[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) h[i] = from_f<T>(v[i]);
         *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(h);
@@ -292,7 +295,7 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 // four of them on one head, joining their sums cost as much as a 1000-token head itself).
 //
 // A warp feeds itself: per page one bulk copy of the head's codes and parameters into one of its two
-// stages while it computes on the other, 16 tokens at a time:
+// stages while it computes on the other, 16 tokens to a tile, two tiles at a time:
 //
 //   S^T [token][row] = K codes (A, 16x16) * q (B, 16x8), on mma.sync.  For 16-bit rows: the code
 //   0..15 in the low bits of a 16-bit word is the f16 subnormal c * 2^-24, exactly, and in the next
@@ -307,7 +310,7 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 // With f32 rows (SPLIT) q and w go in as two f16 each, high and remainder, so that products are good
 // to 2^-22.  mma.sync aligns products by their operands' exponents, of which a subnormal's is above
 // its value, and cuts off what falls below, so f32 rows take the codes as normal numbers, c - 8 (one
-// more instruction for two elements, and less to cancel between scale and offset), and sum 16 tokens
+// more instruction for two elements, and less to cancel between scale and offset), and sum 32 tokens
 // by themselves before the long sum in f32 (4e-6 off without either, 1e-7 with both).  16-bit rows
 // need one operand (an f16 or bf16 q fits f16 after a power of two is taken out; w is rounded to f16,
 // half a step 2^-11, before a sum that is rounded to 16 bits anyway).
@@ -334,6 +337,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t group = a.heads / a.kv_heads, rows = a.queries * group, parts = a.kv_heads * a.tiles;
 
+    pdl_launch_dependents();  // the join may take its place where there is room; it waits for this grid's end
     // ---- where this warp's run of units begins --------------------------------------------------
     if (lane < kKvStages) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(su32(&full[warp][lane])));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -380,10 +384,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
     const uint32_t run = warp * gridDim.x + blockIdx.x;  // neighbouring runs on different SMs
     const unsigned long long first = (unsigned long long)run * per;
     const uint32_t u0 = (uint32_t)min((unsigned long long)total, first), u1 = min(total, u0 + per), units = u1 - u0;
-    if (units == 0) {
-        pdl_launch_dependents();
-        return;
-    }
+    if (units == 0) return;
     Cursor c{0, 0, 0, 0, -1};
     {
         uint32_t lower = 0;  // threads whose sequences begin at or before u0
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
         if (page >= 0)
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                              su32(ring + s * kStageBytes + onto)),
-                         "l"(a.pool + ((size_t)(uint32_t)page * a.kv_heads + at.part / a.tiles) * head_bytes + from),
+                         "l"(a.pool + ((size_t)(uint32_t)page * a.kv_heads + kv_head_of(a, at.part)) * head_bytes + from),
                          "r"(bytes), "r"(su32(&full[warp][s]))
                          : "memory");
     };
@@ -474,7 +475,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
         if (i == 0 || c.chunk == 0) {
             // ---- a new head: its queries as operands, columns 8 n + g --------------------------------
             begun = i;
-            const uint32_t kvh = c.part / a.tiles, tile = c.part % a.tiles;
+            const uint32_t kvh = kv_head_of(a, c.part), tile = c.part - kvh * a.tiles;
             float qs[NT][G];
             int qe[NT];
 #pragma unroll
@@ -486,12 +487,23 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
                          (long long)(kvh * group + r % group) * a.q_head;
                 float x[G * KW][8], top = 0.f;
 #pragma unroll
-                for (uint32_t w = 0; w < G * KW; ++w)  // lane t: words KW t .. of each group
+                for (uint32_t w = 0; w < G * KW; ++w) {  // lane t: words KW t .. of each group
+                    const T* src = qp + (w / KW) * 64 + (KW * t + w % KW) * 8;
+                    alignas(16) T raw[8];
+                    if (qp && a.vec) {
+#pragma unroll
+                        for (uint32_t e = 0; e < sizeof(T) / 2; ++e)
+                            reinterpret_cast<uint4*>(raw)[e] = __ldg(reinterpret_cast<const uint4*>(src) + e);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) raw[e] = qp ? src[e] : from_f<T>(0.f);
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        x[w][e] = qp ? to_f(qp[(w / KW) * 64 + (KW * t + w % KW) * 8 + e]) : 0.f;
+                        x[w][e] = to_f(raw[e]);
                         top = fmaxf(top, fabsf(x[w][e]));
                     }
+                }
 #pragma unroll
                 for (uint32_t gr = 0; gr < G; ++gr) {
                     float sum = 0.f;
@@ -558,90 +570,97 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) l[n][0] = l[n][1] = __int_as_float(0x7fffffff);
         }
-        auto tile16 = [&](uint32_t tok, auto is_edge) {  // 16 tokens from `tok` of the chunk on: within one page
+        // Two tiles of 16 tokens from `tok` of the chunk on, each within one page: twice the independent
+        // work between the votes and the long chains of products.
+        auto tiles32 = [&](uint32_t tok, auto is_edge) {
             constexpr bool kEdge = decltype(is_edge)::value;
-            const uint8_t* base = stage + (tok >> a.page_shift) * stage_head;
-            const uint32_t in_page = tok & (stage_page - 1);
-            const uint8_t* kc = base + in_page * kRow;
-            const uint8_t* kp = base + stage_page * kRow + in_page * (4 * G);
-            const uint8_t* vc = kc + stage_head / 2;
-            const uint8_t* vp = kp + stage_head / 2;
-
-            // S^T
-            float sc[NT][4];
-#pragma unroll
-            for (uint32_t gr = 0; gr < G; ++gr) {
-                uint32_t w0[KW], w1[KW];
-                if (KW == 2) {
-                    const uint2 r0 = *reinterpret_cast<const uint2*>(kc + kt0 * kRow + gr * 32 + t * 8);
-                    const uint2 r1 = *reinterpret_cast<const uint2*>(kc + kt1 * kRow + gr * 32 + t * 8);
-                    w0[0] = r0.x, w0[KW - 1] = r0.y, w1[0] = r1.x, w1[KW - 1] = r1.y;
-                } else {
-                    w0[0] = *reinterpret_cast<const uint32_t*>(kc + kt0 * kRow + t * 4);
-                    w1[0] = *reinterpret_cast<const uint32_t*>(kc + kt1 * kRow + t * 4);
-                }
-                float acc[KW][NT][4];
-#pragma unroll
-                for (uint32_t w = 0; w < KW; ++w) {
-                    uint32_t af[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        codes_of<SPLIT>(h ? w0[w] >> 8 : w0[w], af[h][0], af[h][2]);
-                        codes_of<SPLIT>(h ? w1[w] >> 8 : w1[w], af[h][1], af[h][3]);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const uint32_t f = 2 * (gr * KW + w);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[w][n][e] = 0.f;
-                        if (SPLIT) {  // the small remainders first, before there is a sum to cut them to
-                            mma16816(acc[w][n], af[0], ql[n][f][0], ql[n][f][1]);
-                            mma16816(acc[w][n], af[1], ql[n][f + 1][0], ql[n][f + 1][1]);
-                        }
-                        mma16816(acc[w][n], af[0], qf[n][f][0], qf[n][f][1]);
-                        mma16816(acc[w][n], af[1], qf[n][f + 1][0], qf[n][f + 1][1]);
-                    }
-                }
-                const float2 p0 = params(kp + (kt0 * G + gr) * 4), p1 = params(kp + (kt1 * G + gr) * 4);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 p = e < 2 ? p0 : p1;
-                        const float sum = KW == 2 ? acc[0][n][e] + acc[KW - 1][n][e] : acc[0][n][e];
-                        const float off = p.y * qsum[n][e & 1][gr];
-                        sc[n][e] = fmaf(sum * kfac[n][e & 1], p.x, gr == 0 ? off : off + sc[n][e]);
-                    }
-            }
-            float2 v0[G], v1[G];  // V parameters of this lane's two tokens
-#pragma unroll
-            for (uint32_t gr = 0; gr < G; ++gr) {
-                v0[gr] = params(vp + (kt0 * G + gr) * 4);
-                v1[gr] = params(vp + (kt1 * G + gr) * 4);
-            }
-            const uint32_t t0 = chunk0 + tok + kt0, t1 = t0 + 8;
+            const uint8_t* vc[2];
+            float sc[2][NT][4];
+            float2 v0[2][G], v1[2][G];  // V parameters of this lane's tokens
             // what a column does not see, and what lies behind the sequence, counts for nothing whatever it holds
-            auto hidden = [&](int n, int e) { return kEdge && (int32_t)(e < 2 ? t0 : t1) > last[n][e & 1]; };
-            if (kEdge) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (hidden(n, e)) sc[n][e] = -INFINITY;
-#pragma unroll
-                for (uint32_t gr = 0; gr < G; ++gr) {
-                    if (t0 >= c.len) v0[gr] = make_float2(0.f, 0.f);
-                    if (t1 >= c.len) v1[gr] = make_float2(0.f, 0.f);
-                }
-            }
+            auto hidden = [&](int p, int n, int e) {
+                return kEdge && (int32_t)(chunk0 + tok + 16 * p + (e < 2 ? kt0 : kt1)) > last[n][e & 1];
+            };
             float vtop = 0.f;
 #pragma unroll
-            for (uint32_t gr = 0; gr < G; ++gr) vtop = fmaxf(vtop, fmaxf(v0[gr].x, v1[gr].x));
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t at = tok + 16 * p, in_page = at & (stage_page - 1);
+                const uint8_t* base = stage + (at >> a.page_shift) * stage_head;
+                const uint8_t* kc = base + in_page * kRow;
+                const uint8_t* kp = base + stage_page * kRow + in_page * (4 * G);
+                const uint8_t* vp = kp + stage_head / 2;
+                vc[p] = kc + stage_head / 2;
+                // S^T
+#pragma unroll
+                for (uint32_t gr = 0; gr < G; ++gr) {
+                    uint32_t w0[KW], w1[KW];
+                    if (KW == 2) {
+                        const uint2 r0 = *reinterpret_cast<const uint2*>(kc + kt0 * kRow + gr * 32 + t * 8);
+                        const uint2 r1 = *reinterpret_cast<const uint2*>(kc + kt1 * kRow + gr * 32 + t * 8);
+                        w0[0] = r0.x, w0[KW - 1] = r0.y, w1[0] = r1.x, w1[KW - 1] = r1.y;
+                    } else {
+                        w0[0] = *reinterpret_cast<const uint32_t*>(kc + kt0 * kRow + t * 4);
+                        w1[0] = *reinterpret_cast<const uint32_t*>(kc + kt1 * kRow + t * 4);
+                    }
+                    float acc[KW][NT][4];
+#pragma unroll
+                    for (uint32_t w = 0; w < KW; ++w) {
+                        uint32_t af[2][4];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            codes_of<SPLIT>(h ? w0[w] >> 8 : w0[w], af[h][0], af[h][2]);
+                            codes_of<SPLIT>(h ? w1[w] >> 8 : w1[w], af[h][1], af[h][3]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const uint32_t f = 2 * (gr * KW + w);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[w][n][e] = 0.f;
+                            if (SPLIT) {  // the small remainders first, before there is a sum to cut them to
+                                mma16816(acc[w][n], af[0], ql[n][f][0], ql[n][f][1]);
+                                mma16816(acc[w][n], af[1], ql[n][f + 1][0], ql[n][f + 1][1]);
+                            }
+                            mma16816(acc[w][n], af[0], qf[n][f][0], qf[n][f][1]);
+                            mma16816(acc[w][n], af[1], qf[n][f + 1][0], qf[n][f + 1][1]);
+                        }
+                    }
+                    const float2 p0 = params(kp + (kt0 * G + gr) * 4), p1 = params(kp + (kt1 * G + gr) * 4);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 pp = e < 2 ? p0 : p1;
+                            const float sum = KW == 2 ? acc[0][n][e] + acc[KW - 1][n][e] : acc[0][n][e];
+                            const float off = pp.y * qsum[n][e & 1][gr];
+                            sc[p][n][e] = fmaf(sum * kfac[n][e & 1], pp.x, gr == 0 ? off : off + sc[p][n][e]);
+                        }
+                    v0[p][gr] = params(vp + (kt0 * G + gr) * 4);
+                    v1[p][gr] = params(vp + (kt1 * G + gr) * 4);
+                }
+                if (kEdge) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (hidden(p, n, e)) sc[p][n][e] = -INFINITY;
+#pragma unroll
+                    for (uint32_t gr = 0; gr < G; ++gr) {
+                        if (chunk0 + at + kt0 >= c.len) v0[p][gr] = make_float2(0.f, 0.f);
+                        if (chunk0 + at + kt1 >= c.len) v1[p][gr] = make_float2(0.f, 0.f);
+                    }
+                }
+#pragma unroll
+                for (uint32_t gr = 0; gr < G; ++gr) vtop = fmaxf(vtop, fmaxf(v0[p][gr].x, v1[p][gr].x));
+            }
             bool over = vtop * fv > 64.f || fv == 0.f;
+            float tops[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) over = over || fmaxf(sc[n][j], sc[n][2 + j]) > m[n][j] + 8.f;
+                for (int j = 0; j < 2; ++j) {
+                    tops[n][j] = fmaxf(fmaxf(sc[0][n][j], sc[0][n][2 + j]), fmaxf(sc[1][n][j], sc[1][n][2 + j]));
+                    over = over || tops[n][j] > m[n][j] + 8.f;
+                }
             if (__any_sync(0xffffffffu, over)) {
                 // new references: the rows' maxima, and a power of two that brings w to about 16
                 vtop = warp_max(vtop);
@@ -653,7 +672,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
                     float f[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float top = fmaxf(sc[n][j], sc[n][2 + j]);
+                        float top = tops[n][j];
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                         top = fmaxf(top, m[n][j]);
@@ -670,61 +689,80 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
                 }
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int p = 0; p < 2; ++p)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sc[n][e] = ex2(sc[n][e] - m[n][e & 1]);
-                    l[n][e & 1] += sc[n][e];
-                }
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sc[p][n][e] = ex2(sc[p][n][e] - m[n][e & 1]);
+                        l[n][e & 1] += sc[p][n][e];
+                    }
 
             // O^T
 #pragma unroll
             for (uint32_t gr = 0; gr < G; ++gr) {
-                uint32_t wb[NT][2], wl[NT][2];
-                const float s0 = v0[gr].x * fv, s1 = v1[gr].x * fv;
+                uint32_t wb[2][NT][2], wl[2][NT][2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float x0 = hidden(n, 0) ? 0.f : sc[n][0] * s0, x1 = hidden(n, 1) ? 0.f : sc[n][1] * s0;
-                    const float x2 = hidden(n, 2) ? 0.f : sc[n][2] * s1, x3 = hidden(n, 3) ? 0.f : sc[n][3] * s1;
-                    const uint32_t h0 = pack_h2(x0, x1), h1 = pack_h2(x2, x3);
-                    wb[n][0] = transpose8x8(h0);
-                    wb[n][1] = transpose8x8(h1);
-                    if (SPLIT) {
-                        const float2 r0 = unpack_h2(h0), r1 = unpack_h2(h1);
-                        wl[n][0] = transpose8x8(pack_h2(x0 - r0.x, x1 - r0.y));
-                        wl[n][1] = transpose8x8(pack_h2(x2 - r1.x, x3 - r1.y));
-                    }
+                for (int p = 0; p < 2; ++p) {
+                    const float s0 = v0[p][gr].x * fv, s1 = v1[p][gr].x * fv;
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if (!hidden(n, j)) om[n][j][gr] = fmaf(sc[n][j], v0[gr].y, om[n][j][gr]);
-                        if (!hidden(n, 2 + j)) om[n][j][gr] = fmaf(sc[n][2 + j], v1[gr].y, om[n][j][gr]);
+                    for (int n = 0; n < NT; ++n) {
+                        float x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = hidden(p, n, e) ? 0.f : sc[p][n][e] * (e < 2 ? s0 : s1);
+                        const uint32_t h0 = pack_h2(x[0], x[1]), h1 = pack_h2(x[2], x[3]);
+                        wb[p][n][0] = transpose8x8(h0);
+                        wb[p][n][1] = transpose8x8(h1);
+                        if (SPLIT) {
+                            const float2 r0 = unpack_h2(h0), r1 = unpack_h2(h1);
+                            wl[p][n][0] = transpose8x8(pack_h2(x[0] - r0.x, x[1] - r0.y));
+                            wl[p][n][1] = transpose8x8(pack_h2(x[2] - r1.x, x[3] - r1.y));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            if (!hidden(p, n, j)) om[n][j][gr] = fmaf(sc[p][n][j], v0[p][gr].y, om[n][j][gr]);
+                            if (!hidden(p, n, 2 + j)) om[n][j][gr] = fmaf(sc[p][n][2 + j], v1[p][gr].y, om[n][j][gr]);
+                        }
                     }
                 }
-                // lane g: word g of the group's row (hd 32: half a word), of this lane's four tokens
-                uint32_t w[4];
+                // lane g: word g of the group's row (hd 32: half a word), of this lane's four tokens of each tile
+                uint32_t w[2][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    w[j] = *reinterpret_cast<const uint32_t*>(vc + vt[j] * kRow + gr * 32 + (W == 8 ? g : g >> 1) * 4);
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        w[p][j] = *reinterpret_cast<const uint32_t*>(vc[p] + vt[j] * kRow + gr * 32 + (W == 8 ? g : g >> 1) * 4);
 #pragma unroll
                 for (uint32_t hw = 0; hw < W / 4; ++hw) {  // 16-bit halves of the words: dims 4 hw ..
                     const uint32_t sel = W == 8 ? (hw ? 0x7632u : 0x5410u) : (g & 1 ? 0x7632u : 0x5410u);
-                    const uint32_t a0 = __byte_perm(w[0], w[1], sel), a1 = __byte_perm(w[2], w[3], sel);
+                    uint32_t a0[2], a1[2];
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        a0[p] = __byte_perm(w[p][0], w[p][1], sel);
+                        a1[p] = __byte_perm(w[p][2], w[p][3], sel);
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        uint32_t af[4];
-                        codes_of<SPLIT>(h ? a0 >> 8 : a0, af[0], af[1]);
-                        codes_of<SPLIT>(h ? a1 >> 8 : a1, af[2], af[3]);
+                        uint32_t af[2][4];
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            codes_of<SPLIT>(h ? a0[p] >> 8 : a0[p], af[p][0], af[p][1]);
+                            codes_of<SPLIT>(h ? a1[p] >> 8 : a1[p], af[p][2], af[p][3]);
+                        }
                         const uint32_t d = gr * 4 + 2 * hw + h;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            if (SPLIT) {  // 16 tokens' sum by itself: the long one is rounded, not cut, in f32
+                            if (SPLIT) {  // 32 tokens' sum by itself: the long one is rounded, not cut, in f32
                                 float add[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma16816(add, af, wl[n][0], wl[n][1]);
-                                mma16816(add, af, wb[n][0], wb[n][1]);
+#pragma unroll
+                                for (int p = 0; p < 2; ++p) mma16816(add, af[p], wl[p][n][0], wl[p][n][1]);
+#pragma unroll
+                                for (int p = 0; p < 2; ++p) mma16816(add, af[p], wb[p][n][0], wb[p][n][1]);
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) o[n][d][e] += add[e];
                             } else {
-                                mma16816(o[n][d], af, wb[n][0], wb[n][1]);
+#pragma unroll
+                                for (int p = 0; p < 2; ++p) mma16816(o[n][d], af[p], wb[p][n][0], wb[p][n][1]);
                             }
                         }
                     }
@@ -733,10 +771,10 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
         };
         if (!edge) {
 #pragma unroll 1
-            for (uint32_t tok = 0; tok < kKvChunk; tok += 16) tile16(tok, std::false_type{});
+            for (uint32_t tok = 0; tok < kKvChunk; tok += 32) tiles32(tok, std::false_type{});
         } else {
 #pragma unroll 1
-            for (uint32_t tok = 0; tok < kKvChunk && chunk0 + tok < c.len; tok += 16) tile16(tok, std::true_type{});
+            for (uint32_t tok = 0; tok < kKvChunk && chunk0 + tok < c.len; tok += 32) tiles32(tok, std::true_type{});
         }
         __syncwarp();  // every lane has read the stage
         if (fetched < units) fetch_next();
@@ -745,7 +783,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
         if (head_done || i + 1 == units) {
             // ---- the head's result, or this run's part of it --------------------------------------------
             const float back = fv == 0.f ? 0.f : kUp / fv;
-            const uint32_t kvh = c.part / a.tiles, tile = c.part % a.tiles;
+            const uint32_t kvh = kv_head_of(a, c.part), tile = c.part - kvh * a.tiles;
             const bool whole = head_done && i - begun == c.chunk;
             // the run's first head goes to slot 0 of its two, one that began later to slot 1
             float* part = a.part + (size_t)(2 * run + (begun ? 1 : 0)) * kCols * (HD + 4);
@@ -810,17 +848,16 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
         for (uint32_t i = fetched > kKvStages ? fetched - kKvStages : 0; i < fetched; ++i)
             mbar_wait(&full[warp][i % kKvStages], (i / kKvStages) & 1, kKvSpin);
     }
-    pdl_launch_dependents();
 }
 
 // Joins the partial results of the heads that more than one run shared, in the order of the runs,
-// and writes zeros for sequences of length 0.  A block per (sequence, kv head, row tile) and share of
-// its rows; 4 dims a thread, the runs' pieces over the rest of the block.
-template <typename T, int HD, int NT>
+// and writes zeros for sequences of length 0.  A block per (sequence, kv head, row tile) and COLS of
+// its rows; a thread has 4 dims of one row, the rest of the block shares the pieces.
+template <typename T, int HD, int NT, int COLS>
 __global__ void __launch_bounds__(256) k_kv4_join(AttnArgs a) {
-    constexpr uint32_t kCols = 8 * NT, kLanes = HD / 4, kSplit = 256 / kLanes;
-    __shared__ float4 s_acc[256];
-    __shared__ float s_l[kSplit], s_red[8];
+    constexpr uint32_t kCols = 8 * NT, kLanes = HD / 4, kSplit = 256 / kLanes / COLS;
+    __shared__ float4 s_acc[kSplit][COLS * kLanes];
+    __shared__ float s_l[kSplit][COLS], s_top[kSplit][COLS];
     pdl_wait();
     const uint32_t group = a.heads / a.kv_heads, rows = a.queries * group, tid = threadIdx.x;
     const uint32_t parts = a.kv_heads * a.tiles, part = blockIdx.x % parts, b = blockIdx.x / parts;
@@ -832,50 +869,51 @@ __global__ void __launch_bounds__(256) k_kv4_join(AttnArgs a) {
     const uint32_t u0 = a.head_ws[b] + part * n, u1 = u0 + n;
     const uint32_t c0 = u0 / per, c1 = len ? (u1 - 1) / per : c0 + 1;
     if (c0 == c1) return;  // one run had it all
-    const uint32_t kvh = part / a.tiles, r0 = part % a.tiles * kCols;
-    for (uint32_t col = blockIdx.y; col < kCols && r0 + col < rows; col += gridDim.y) {
-        const uint32_t r = r0 + col;
-        T* dst = static_cast<T*>(a.out) + (((size_t)b * a.queries + r / group) * a.heads + kvh * group + r % group) * HD;
-        if (len == 0) {
-            if (tid < HD) dst[tid] = from_f<T>(0.f);
-            continue;
-        }
+    const uint32_t kvh = part / a.tiles, d4 = tid % kLanes, local = tid / kLanes % COLS, share = tid / kLanes / COLS;
+    const uint32_t col = blockIdx.y * COLS + local, r = part % a.tiles * kCols + col;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float ls = 0.f;
+    if (len) {
         // run c's piece begins at its own first unit (slot 0) or, only for c0, behind it (slot 1)
         auto piece = [&](uint32_t c) {
             return a.part + ((size_t)(2 * c + (u0 > c * per ? 1 : 0)) * kCols + col) * (HD + 4);
         };
         float top = kKvLow;
-        for (uint32_t c = c0 + tid; c <= c1; c += 256) top = fmaxf(top, piece(c)[HD]);
-        top = warp_max(top);
-        __syncthreads();  // the last row's shared values have been read
-        if ((tid & 31) == 0) s_red[tid >> 5] = top;
+        if (r < rows) {
+#pragma unroll 4
+            for (uint32_t c = c0 + share; c <= c1; c += kSplit) top = fmaxf(top, piece(c)[HD]);
+        }
+        if (d4 == 0) s_top[share][local] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 8; ++w) top = fmaxf(top, s_red[w]);
-        const uint32_t d4 = tid % kLanes, share = tid / kLanes;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        float ls = 0.f;
+        for (uint32_t p = 0; p < kSplit; ++p) top = fmaxf(top, s_top[p][local]);
+        if (r < rows) {
 #pragma unroll 4
-        for (uint32_t c = c0 + share; c <= c1; c += kSplit) {
-            const float* p = piece(c);
-            const float f = ex2(p[HD] - top);
-            const float4 v = reinterpret_cast<const float4*>(p)[d4];
-            sum = make_float4(fmaf(f, v.x, sum.x), fmaf(f, v.y, sum.y), fmaf(f, v.z, sum.z), fmaf(f, v.w, sum.w));
-            ls = fmaf(f, p[HD + 1], ls);
-        }
-        s_acc[tid] = sum;
-        if (d4 == 0) s_l[share] = ls;
-        __syncthreads();
-        if (tid < HD) {
-            float total = 0.f, lt = 0.f;
-#pragma unroll 8
-            for (uint32_t p = 0; p < kSplit; ++p) {
-                total += reinterpret_cast<const float*>(s_acc)[p * HD + tid];
-                lt += s_l[p];
+            for (uint32_t c = c0 + share; c <= c1; c += kSplit) {
+                const float* p = piece(c);
+                const float f = ex2(p[HD] - top);
+                const float4 v = reinterpret_cast<const float4*>(p)[d4];
+                sum = make_float4(fmaf(f, v.x, sum.x), fmaf(f, v.y, sum.y), fmaf(f, v.z, sum.z), fmaf(f, v.w, sum.w));
+                ls = fmaf(f, p[HD + 1], ls);
             }
-            dst[tid] = from_f<T>(lt == 0.f ? 0.f : total / lt);
         }
+        s_acc[share][tid % (COLS * kLanes)] = sum;
+        if (d4 == 0) s_l[share][local] = ls;
+        __syncthreads();
     }
+    if (share || r >= rows) return;
+#pragma unroll 4
+    for (uint32_t p = 1; p < kSplit && len; ++p) {
+        const float4 v = s_acc[p][tid];
+        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+        ls += s_l[p][local];
+    }
+    const float inv = ls == 0.f ? 0.f : 1.f / ls;
+    T* dst = static_cast<T*>(a.out) + (((size_t)b * a.queries + r / group) * a.heads + kvh * group + r % group) * HD + d4 * 4;
+    dst[0] = from_f<T>(sum.x * inv);
+    dst[1] = from_f<T>(sum.y * inv);
+    dst[2] = from_f<T>(sum.z * inv);
+    dst[3] = from_f<T>(sum.w * inv);
 }
 
 // ---- launches -----------------------------------------------------------------------------------
@@ -912,16 +950,17 @@ cudaError_t launch_attn4(AttnArgs a, uint64_t most_units, cudaStream_t st) {
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
-    // few heads: a block per row, as their pieces are many; else a block for all rows of a tile
+    // few heads: a block per row, as their pieces are many; else blocks of 8 rows (which hd 128 fills)
     const uint32_t heads = a.batch * a.kv_heads * a.tiles;
-    cfg.gridDim = dim3(heads, heads <= 148 ? 8 * NT : 1);
+    const bool few = heads <= 148;
+    cfg.gridDim = dim3(heads, few ? 8 * NT : NT);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_kv4_join<T, HD, NT>, a);
+    return few ? cudaLaunchKernelEx(&cfg, k_kv4_join<T, HD, NT, 1>, a) : cudaLaunchKernelEx(&cfg, k_kv4_join<T, HD, NT, 8>, a);
 }
 
 template <typename T, bool SPLIT>
@@ -1039,6 +1078,9 @@ extern "C" enx_status enx_attn_kv4(const void* q, const int64_t* strides, const 
     a.page_shift = log2_of(d->page_tokens);
     a.tiles = tiles;
     a.most_chunks = (uint32_t)chunks;
+    uintptr_t any = reinterpret_cast<uintptr_t>(q);
+    for (int i = 0; i < 3; ++i) any |= (uintptr_t)strides[i] * (d->dtype == ENX_F32 ? 4 : 2);
+    a.vec = any % 16 == 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     if (d->dtype == ENX_F32)
         ENX_CUDA((pick_attn4<float, true>(a, d->head_dim, nt, units, as_stream(stream))));

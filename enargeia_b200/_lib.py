@@ -113,6 +113,7 @@ SIGNATURES = {
     "enx_kv4_write": (C.c_int32, [P, P, C.POINTER(C.c_int64), U32, P, P, P, P, P, P, C.POINTER(Kv4Dims), P]),
     "enx_attn_kv4": (C.c_int32, [P, C.POINTER(C.c_int64), P, P, P, P, P, U32, U32, U32, F32, C.POINTER(Kv4Dims), P, P]),
     "enx_attn_kv4_workspace_bytes": (C.c_size_t, [U32, U32]),
+    "enx_attn_packed": (C.c_int32, [P, P, P, P, C.POINTER(C.c_int64), P, U32, U32, U32, U32, U32, U32, F32, P]),
     "enx_create": (C.c_int32, [C.POINTER(ModelConfigC), C.c_int, C.POINTER(P)]),
     "enx_destroy": (C.c_int32, [P]),
     "enx_load_enargeia": (C.c_int32, [P, C.c_char_p]),

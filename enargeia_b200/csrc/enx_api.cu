@@ -18,6 +18,7 @@
 #include "k_gemm_tc.cuh"
 #include "k_kv4.cuh"
 #include "k_mega.cuh"
+#include "k_packed.cuh"
 #include "k_small.cuh"
 #include "json_lite.h"
 
@@ -93,9 +94,11 @@ extern "C" enx_status enx_raw_check(void) {
     int dev = 0;
     ENX_CUDA(cudaGetDevice(&dev));
     ENX_CUDA(cudaDeviceSynchronize());
-    uint32_t waited = 0;
-    ENX_CUDA(kv4_take_error(&waited));
-    if (waited) return fail(ENX_ERR_TIMEOUT, "enx_attn_kv4: a bounded device wait gave up");
+    uint32_t kv4 = 0, packed = 0;
+    ENX_CUDA(kv4_take_error(&kv4));
+    ENX_CUDA(packed_take_error(&packed));
+    if (kv4 || packed)
+        return fail(ENX_ERR_TIMEOUT, std::string(kv4 ? "enx_attn_kv4" : "enx_attn_packed") + ": a bounded device wait gave up");
     uint32_t* err = nullptr;
     {
         std::lock_guard<std::mutex> lock(g_tc_mu);
@@ -120,6 +123,7 @@ extern "C" enx_status enx_set_wait_limit(int device, uint32_t spins) {
     cudaError_t e = mega_set_spin(spins);
     if (e == cudaSuccess) e = tc_set_spin(spins);
     if (e == cudaSuccess) e = kv4_set_spin(spins);
+    if (e == cudaSuccess) e = packed_set_spin(spins);
     cudaSetDevice(prev);
     ENX_CUDA(e);
     return ENX_OK;

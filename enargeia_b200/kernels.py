@@ -310,6 +310,28 @@ def attn_kv4(q, pool, table, lengths, out, kv_heads, page_tokens, seqs=None, sca
     return out
 
 
+def attn_packed(q, k, v, out, offsets, scale=None, stream=None):
+    """Causal attention over prompts packed one behind another: q and out [tokens, heads, head_dim], k
+    and v [tokens, kv_heads, head_dim], float16 or bfloat16, any strides whose rows start on 16 bytes;
+    prompt s has rows offsets[s] to offsets[s + 1] - 1 (int32 on the device)."""
+    tokens, heads, hd = q.shape
+    kv_heads = k.shape[1]
+    if q.dtype is not torch.float16 and q.dtype is not torch.bfloat16:
+        raise ValueError(f"expected float16 or bfloat16, got {q.dtype}")
+    if out.shape != q.shape or k.shape != (tokens, kv_heads, hd) or v.shape != k.shape:
+        raise ValueError("q and out have to have one shape, and k and v one with the same tokens and head_dim")
+    if not (q.dtype is k.dtype is v.dtype is out.dtype):
+        raise ValueError("q, k, v and out have to have one type")
+    strides = (C.c_int64 * 8)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                              out.stride(0), out.stride(1))
+    if offsets.numel() < 1:
+        raise ValueError("offsets has an entry more than there are prompts")
+    _call_on((q, k, v, out, offsets), "enx_attn_packed", _rows_of(q), _rows_of(k), _rows_of(v), _rows_of(out), strides,
+             _i32(offsets, None), offsets.numel() - 1, tokens, heads, kv_heads, hd, _DTYPES[q.dtype],
+             hd ** -0.5 if scale is None else scale, stream=stream)
+    return out
+
+
 def to_device_u32(a) -> torch.Tensor:
     """numpy uint32 -> CUDA int32 tensor with the same bits."""
     import numpy as np

@@ -79,8 +79,8 @@ ENX_API enx_status enx_matmul_q4(const float* x, const uint32_t* packed, const f
  * enx_raw_check reads it. */
 
 /* Report (then clear) the sticky error word of the raw tensor-core entry points and of
- * enx_attn_kv4: ENX_ERR_TIMEOUT if a bounded wait gave up since the last check, whose outputs are
- * then invalid.  It first waits for ALL work on the current device (cudaDeviceSynchronize), including
+ * enx_attn_kv4 and enx_attn_packed: ENX_ERR_TIMEOUT if a bounded wait gave up since the last check,
+ * whose outputs are then invalid.  It first waits for ALL work on the current device (cudaDeviceSynchronize), including
  * the streams of other enx contexts and of other libraries on that device, so it must not be
  * called while any stream of the device is being captured into a CUDA graph.  No reference
  * counterpart (WebGPU kernels have no device waits). */
@@ -330,6 +330,21 @@ ENX_API enx_status enx_attn_kv4(const void* q, const int64_t* strides, const uin
                                 void* out, uint32_t batch, uint32_t queries, uint32_t heads,
                                 float scale, const enx_kv4_dims* dims, void* workspace, void* stream);
 ENX_API size_t enx_attn_kv4_workspace_bytes(uint32_t batch, uint32_t head_dim);
+
+/* Causal attention over whole prompts packed one behind another (the reference prefills one
+ * sequence, in f32 over its f16 cache: src/kernels/cache_variants.ts:81-144): token i of prompt s
+ * (rows offsets[s] to offsets[s + 1] - 1; offsets int32 [seqs + 1] on the device, ascending) attends the
+ * tokens of its prompt up to itself, softmax of scale * q.k.  q and out are [tokens][heads][head_dim],
+ * k and v [tokens][kv_heads][head_dim], heads a multiple of kv_heads; strides[0..7] are the token and
+ * head strides, in elements, of q, k, v and out, whose rows start on 16 bytes.  dtype ENX_F16 or
+ * ENX_BF16; head_dim a multiple of 8, at most 128.  Rows of no prompt are left as they were, and no
+ * row depends on one it does not attend, whatever that holds.  Scores, softmax and sums in f32, weights
+ * rounded to the dtype for their product with v.  No workspace.  enx_raw_check reports a bounded wait
+ * that gave up. */
+ENX_API enx_status enx_attn_packed(const void* q, const void* k, const void* v, void* out,
+                                   const int64_t* strides, const int32_t* offsets, uint32_t seqs,
+                                   uint32_t tokens, uint32_t heads, uint32_t kv_heads,
+                                   uint32_t head_dim, uint32_t dtype, float scale, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Model context: WeightStore + KVCache + DecodeGraph + ForwardGraph + Session's step.

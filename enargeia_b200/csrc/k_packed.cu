@@ -3,10 +3,10 @@
 //
 // out[i] = sum_j softmax_j(scale * q[i].k[j]) v[j] over the keys j <= i of token i's own prompt.
 //
-// A CTA owns 256 consecutive queries of one prompt and head, as two tiles of 128 rows that take turns:
-// while one warpgroup turns the first tile's scores into weights, the tensor cores multiply for the
-// second.  Keys go by in tiles of 128, counted from the prompt's start like the rows, so that of each
-// row tile only the last key tile needs a mask.  Per key tile and row tile:
+// An item of work is 256 consecutive queries of one prompt and head, as two tiles of 128 rows that take
+// turns: while one warpgroup turns the first tile's scores into weights, the tensor cores multiply for
+// the second.  Keys go by in tiles of 128, counted from the prompt's start like the rows, so that of
+// each row tile only the last key tile needs a mask.  Per key tile and row tile:
 //
 //   S (TMEM, f32) = Q K^T           kind::f16, M = N = 128, both operands K-major from shared memory
 //   p = 2^(scale' (s - m)), to TMEM over S, in 16 bits
@@ -16,19 +16,26 @@
 // more than 2^8 in its weight; then the warpgroup rescales its rows of O in TMEM, which is rare.  Sums
 // are f32.  Weights are rounded to the inputs' 16 bits for the product, as the output is.
 //
-// Bound: one exponential per score against 4 hd multiply-adds.  16 a clock and SM make 1024 clocks per
-// 128 x 128 scores, the products 512 at hd 64 and 1024 at hd 128.
+// Bound: one exponential per score against 4 hd multiply-adds.  At 16 a clock and SM, 128 x 128 scores
+// are 1024 clocks, their products 512 at hd 64 and 1024 at hd 128; so three of eight exponentials are
+// taken on the FMA pipe instead (2^x = 2^n 2^f, a cubic in f).
+//
+// One CTA per SM works through items, the next one's loads and first products under the present one's
+// last weights and output.  Items are in descending order of their key tiles, over all prompts and
+// heads, and dealt out to and fro (CTA c takes items c, 2G - 1 - c, 2G + c, ..), which keeps the CTAs'
+// shares even without a counter.
 //
 // Warp roles, synchronised by mbarriers with bounded waits:
-//   warps 0-3, 4-7  softmax of row tile 0 and 1 (thread = row), then its output
-//   warp 8          TMEM; lane 0 issues all products
-//   warp 9          lane 0 loads Q, K and V tiles by TMA (128-byte swizzle; 64-element halves of a row)
-//   warps 10, 11    look through the V tiles that some row sees only in part (see below)
+//   warps 0-3, 4-7  softmax of row tile 0 and 1 (thread = row)
+//   warps 8-11      output of both row tiles; and the V tiles that some row sees only in part (below)
+//   warps 12, 15    lane 0 issues the products of row tile 0 and 1 (and warp 12 owns TMEM)
+//   warp 13         lane 0 loads Q, K and V tiles by TMA (128-byte swizzle; 64-element halves of a row)
+//   warp 14         finds the items
 //
-// A weight of zero times a V element that is not finite would be NaN.  The last two key tiles of a CTA
-// are the only ones that hold keys which some row does not see, so in those the helper warps replace such
-// elements by zeros before the product, and where there were any, each row adds those that it does see
-// when it writes its output.
+// A weight of zero times a V element that is not finite would be NaN.  The last two key tiles of an item
+// are the only ones that hold keys which some row does not see, so in those the output warps replace
+// such elements by zeros before the product, and where there were any, each row adds those that it does
+// see to its output.
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -47,10 +54,12 @@ __device__ uint32_t g_packed_spin = kPkSpin;
 __device__ uint32_t g_packed_err = 0;
 
 constexpr uint32_t kPkRows = 128;           // rows of a tile, keys of a tile
-constexpr uint32_t kPkThreads = 384;
+constexpr uint32_t kPkThreads = 512;
+constexpr uint32_t kPkItems = 4;             // items between the warp that finds them and the others
+constexpr uint32_t kPkClean = 4;             // barriers of partly seen V tiles: more than a ring holds
 constexpr uint32_t kPkTileBytes = 128 * 128;  // 128 rows of 64 16-bit elements
-constexpr int kPkRegs = 168, kPkRegsSoftmax = 224, kPkRegsRest = 56;
-static_assert(2 * kPkRegsSoftmax + kPkRegsRest <= 3 * kPkRegs, "the warpgroups' registers come out of the launch's");
+constexpr int kPkRegs = 128, kPkRegsSoftmax = 192, kPkRegsOut = 80, kPkRegsRest = 48;
+static_assert(2 * kPkRegsSoftmax + kPkRegsOut + kPkRegsRest <= 4 * kPkRegs, "the warpgroups' registers come out of the launch's");
 
 template <int D>
 struct PackedShape {
@@ -108,13 +117,13 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 
 // Shared-memory matrix descriptors of tiles written by TMA with the 128-byte swizzle: rows of 128
 // bytes, 8-row groups 1024 bytes apart.  K-major (Q, K): the next 16 elements of a row are 32 bytes on.
-// MN-major (V): the next 16 keys are 2048 bytes on, the next 64 dims a tile half (16 KB).
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// MN-major (V): the next 16 keys are 2048 bytes on, the next 64 dims a tile half (16 KB).  addr16: the
+// address in units of 16 bytes (below 2^14: shared memory).
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr16) {
+    return (uint64_t)(addr16 | (1u << 16)) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(kPkTileBytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr16) {
+    return (uint64_t)(addr16 | ((kPkTileBytes >> 4) << 16)) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
 // f32 accumulators, both operands f16 or both bf16; B K-major or MN-major.
@@ -178,6 +187,13 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The largest of three, NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
@@ -209,6 +225,31 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
     return r;
 }
 
+// 2^x for two x <= 9: x = n + f with n the nearest whole number (the low bits of x + 1.5 * 2^23),
+// 2^f by the cubic with the least relative error on [-1/2, 1/2] (Remez exchange: 7.5e-5, below the
+// weights' rounding to 16 bits), n added to its exponent.  x is cut at -126, where 2^x counts for nothing.
+__device__ __forceinline__ void ex2_poly(Pair xy, float& a, float& b) {
+    float x, y;
+    unpair(xy, x, y);
+    xy = pair(fmaxf(x, -126.f), fmaxf(y, -126.f));
+    const Pair big = pair(12582912.f, 12582912.f), nbig = pair(-12582912.f, -12582912.f), one = pair(-1.f, -1.f);
+    const Pair n = add2(xy, big);
+    const Pair f = fma2(add2(n, nbig), one, xy);
+    Pair r = fma2(pair(0x1.c3f760p-5f, 0x1.c3f760p-5f), f, pair(0x1.f0de1ap-3f, 0x1.f0de1ap-3f));
+    r = fma2(r, f, pair(0x1.62f31ap-1f, 0x1.62f31ap-1f));
+    r = fma2(r, f, pair(0x1.fff692p-1f, 0x1.fff692p-1f));
+    float nx, ny;
+    unpair(n, nx, ny);
+    unpair(r, a, b);
+    a = __int_as_float(__float_as_int(a) + (__float_as_int(nx) << 23));
+    b = __int_as_float(__float_as_int(b) + (__float_as_int(ny) << 23));
+}
+
+// Rows [begin, begin + len) of the packed tensors, the pair-th 256 of them, of one head; len 0: no more.
+struct Item {
+    uint32_t begin, len, pair, head;
+};
+
 // A 16-bit element whose exponent bits are all ones
 template <bool BF16>
 __device__ __forceinline__ bool not_finite16(uint32_t x) {
@@ -226,72 +267,48 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     constexpr uint32_t kStages = Sh::kStages, kTile = Sh::kTile, kHalves = Sh::kHalves;
     constexpr uint32_t kTmemO = 256;  // columns: S (and P) of the two row tiles, then O of each
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t q_full, kv_full[kStages], kv_empty[kStages], v_raw[2], v_clean[2], s_full[2], p_full[2], o_full[2];
-    __shared__ uint32_t tmem_base, s_seq[3];
+    __shared__ __align__(8) uint64_t kv_full[kStages], kv_empty[kStages], v_raw[kPkClean], v_clean[kPkClean];
+    __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], l_full[2], o_empty[2], drain[2];
+    __shared__ __align__(8) uint64_t it_full[kPkItems], it_empty[kPkItems];
+    __shared__ Item s_item[kPkItems];
+    __shared__ float s_inv[2][128];
+    __shared__ uint32_t tmem_base;
     __shared__ volatile int s_fail;
-    __shared__ int s_foul;  // a V element that is not finite among the last two key tiles
+    __shared__ uint32_t s_foul;  // 1 + the last item in whose partly seen V tiles an element was not finite
 
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.y;
-
-    // ---- which prompt and which 256 rows: tile blockIdx.x of all prompts' tiles, long ones first ------
-    if (warp == 0) {
-        uint32_t before = 0, found = 0, begin = 0, len = 0, back = 0;
-        for (uint32_t s0 = 0; s0 < a.seqs && !found; s0 += 32) {
-            const uint32_t s = s0 + lane;
-            uint32_t b = 0, n = 0;
-            if (s < a.seqs) {
-                b = (uint32_t)min(max(a.offsets[s], 0), (int32_t)a.tokens);
-                const uint32_t e = (uint32_t)min(max(a.offsets[s + 1], 0), (int32_t)a.tokens);
-                n = e > b ? e - b : 0;
-            }
-            const uint32_t tiles = (n + 255) / 256;
-            uint32_t incl = tiles;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= (uint32_t)o) incl += up;
-            }
-            const uint32_t lo = before + incl - tiles;
-            const uint32_t hit = __ballot_sync(0xffffffffu, blockIdx.x >= lo && blockIdx.x < lo + tiles);
-            if (hit) {
-                const int src = __ffs(hit) - 1;
-                begin = __shfl_sync(0xffffffffu, b, src);
-                len = __shfl_sync(0xffffffffu, n, src);
-                back = blockIdx.x - __shfl_sync(0xffffffffu, lo, src);
-                found = 1;
-            }
-            before += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (lane == 0) {
-            s_seq[0] = begin;
-            s_seq[1] = found ? len : 0;
-            s_seq[2] = found ? (len + 255) / 256 - 1 - back : 0;
-        }
-    }
-    if (tid == 32) {
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
         s_fail = 0;
         s_foul = 0;
         auto init = [](uint64_t* bar, uint32_t count) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(bar)), "r"(count));
         };
-        init(&q_full, 1);
         for (uint32_t i = 0; i < kStages; ++i) {
             init(&kv_full[i], 1);
-            init(&kv_empty[i], 1);
+            init(&kv_empty[i], 2);  // both row tiles
+        }
+        for (uint32_t i = 0; i < kPkClean; ++i) {
+            init(&v_raw[i], 1);
+            init(&v_clean[i], 128);
+        }
+        for (uint32_t i = 0; i < kPkItems; ++i) {
+            init(&it_full[i], 1);
+            init(&it_empty[i], 15);  // 8 softmax warps, 4 output warps, 2 of products, loads
         }
         for (int i = 0; i < 2; ++i) {
-            init(&v_raw[i], 1);
-            init(&v_clean[i], 64);
+            init(&q_full[i], 1);
+            init(&q_empty[i], 1);
             init(&s_full[i], 1);
-            init(&p_full[i], 128);
+            init(&p_full[i][0], 128);
+            init(&p_full[i][1], 128);
             init(&o_full[i], 1);
+            init(&l_full[i], 128);
+            init(&o_empty[i], 128);
+            init(&drain[i], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
-    const uint32_t begin = s_seq[0], len = s_seq[1], pair_tile = s_seq[2];
-    if (len == 0) return;  // the grid covers the most tiles that the offsets could make
-    if (warp == 8) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&tmem_base)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -301,238 +318,144 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     const uint32_t tmem = tmem_base, limit = g_packed_spin;
     const uint32_t smem = (su32(smem_raw) + 1023) & ~1023u;
     const uint32_t sq = smem, skv = smem + 2 * kTile;
-    const uint32_t kvh = head / (a.heads / a.kv_heads);
-    const uint32_t first_row = pair_tile * 256;  // of the prompt
+    const uint32_t group = a.heads / a.kv_heads;
+    auto wait = [&](uint64_t* bar, uint32_t phase) { return mbar_wait_f(bar, phase & 1, &s_fail, limit); };
+    // The k-th item of this CTA, read by a whole warp or (one) by a single thread.
+    auto next_item = [&](uint32_t k, Item& it, bool one) {
+        bool ok = wait(&it_full[k % kPkItems], k / kPkItems);
+        if (!one) ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return false;
+        it = s_item[k % kPkItems];
+        if (!one) __syncwarp();
+        if (one || lane == 0) mbar_arrive(&it_empty[k % kPkItems]);
+        return it.len != 0;
+    };
     // key tiles of each row tile: up to the one on its diagonal
-    const uint32_t n0 = 2 * pair_tile + 1, n1 = first_row + 128 < len ? n0 + 1 : 0, n = max(n0, n1);
+    auto tiles0 = [](const Item& it) { return 2 * it.pair + 1; };
+    auto tiles1 = [](const Item& it) { return it.pair * 256 + 128 < it.len ? 2 * it.pair + 2 : 0; };
 
     if (warp < 8) {
         // ---- softmax of row tile w: thread = row ---------------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPkRegsSoftmax));
-        const uint32_t w = warp >> 2, row = tid & 127, tiles = w ? n1 : n0;
+        const uint32_t w = warp >> 2, row = tid & 127;
         const uint32_t lanes = (32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + w * 128, to = tmem + lanes + kTmemO + w * D;
         const float c = a.scale_log2;
-        float m = 0.f;
-        Pair l2 = pair(0.f, 0.f), l3 = l2;
+        uint32_t steps = 0, done = 0;  // key tiles and items of this row tile so far
         bool ok = true;
-        for (uint32_t j = 0; j < tiles; ++j) {
-            if (!mbar_wait_f(&s_full[w], j & 1, &s_fail, limit)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            fence_after();
-            uint32_t s[4][32];
+        Item it;
+        for (uint32_t k = 0; ok && next_item(k, it, false); ++k) {
+            const uint32_t tiles = w ? tiles1(it) : tiles0(it);
+            if (!tiles) continue;
+            float m = 0.f;
+            Pair l2 = pair(0.f, 0.f), l3 = l2;
+            for (uint32_t j = 0; j < tiles; ++j, ++steps) {
+                ok = __all_sync(0xffffffffu, wait(&s_full[w], steps));
+                if (!ok) break;
+                fence_after();
+                uint32_t s[4][32];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld32(s[i], ts + 32 * i);
-            tmem_wait_ld();
-            if (j + 1 == tiles) {  // the diagonal: key column > row is not seen
+                for (int i = 0; i < 4; ++i) tmem_ld32(s[i], ts + 32 * i);
+                tmem_wait_ld();
+                if (j + 1 == tiles) {  // the diagonal: key column > row is not seen
 #pragma unroll
-                for (int i = 0; i < 128; ++i)
-                    if ((uint32_t)i > row) s[i / 32][i % 32] = 0xff800000u;
-            }
-            float top[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                top[i] = __uint_as_float(s[i][0]);
-#pragma unroll
-                for (int k = 1; k < 32; ++k) top[i] = fmaxf(top[i], __uint_as_float(s[i][k]));
-            }
-            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            if (j == 0) {
-                m = mx;
-            } else if (__any_sync(0xffffffffu, (mx - m) * c > 8.f)) {
-                const float m_new = fmaxf(m, mx), f = m_new == -INFINITY ? 1.f : ex2((m - m_new) * c);
-                m = m_new;
-                float x, y;
-                unpair(l2, x, y);
-                l2 = pair(x * f, y * f);
-                unpair(l3, x, y);
-                l3 = pair(x * f, y * f);
-                // the product of the last key tile is complete: this tile's scores were issued after it
-#pragma unroll 1
-                for (uint32_t k = 0; k < D; k += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(o, to + k);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                    tmem_st32(to + k, o);
+                    for (int i = 0; i < 128; ++i)
+                        if ((uint32_t)i > row) s[i / 32][i % 32] = 0xff800000u;
                 }
-            }
-            const float mc = m == -INFINITY ? 0.f : -m * c;
-            const Pair cc = pair(c, c), mm = pair(mc, mc);
+                float top[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t p[32];
+                for (int i = 0; i < 4; ++i) {
+                    top[i] = __uint_as_float(s[i][0]);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const uint32_t e = 64 * h + 2 * i;
+                    for (int e = 1; e < 31; e += 2) top[i] = max3(top[i], __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+                }
+                float mx = max3(top[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
+                mx = max3(mx, __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
+                mx = max3(max3(mx, top[1], top[2]), top[3], mx);
+                // NaN among the scores stays NaN in the maximum, and infinity makes one, as inf - inf: the
+                // whole row is NaN then, whichever way its exponentials are taken
+                if (mx == INFINITY) mx = __int_as_float(0x7fffffff);
+                const bool move = j == 0 || !((mx - m) * c <= 8.f);
+                if (j == 0) {
+                    m = mx;
+                } else if (__any_sync(0xffffffffu, move)) {  // each row by itself: none depends on its neighbours
+                    const float m_new = move ? max3(m, mx, mx) : m, f = move && m_new != -INFINITY ? ex2((m - m_new) * c) : 1.f;
+                    m = m_new;
                     float x, y;
-                    unpair(fma2(pair(__uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1])), cc, mm), x, y);
-                    x = ex2(x);
-                    y = ex2(y);
-                    if (i & 1)
-                        l3 = add2(l3, pair(x, y));
-                    else
-                        l2 = add2(l2, pair(x, y));
-                    p[i] = pack2<BF16>(x, y);
+                    unpair(l2, x, y);
+                    l2 = pair(x * f, y * f);
+                    unpair(l3, x, y);
+                    l3 = pair(x * f, y * f);
+                    // the product of the last key tile is complete: this tile's scores were issued after it
+#pragma unroll 1
+                    for (uint32_t d = 0; d < D; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o, to + d);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st32(to + d, o);
+                    }
                 }
-                tmem_st32(ts + 32 * h, p);
+                const float mc = m == -INFINITY ? 0.f : -m * c;
+                const Pair cc = pair(c, c), mm = pair(mc, mc);
+                // weights i0 .. i0 + n of the row's 64 pairs, into p
+                auto weights = [&](uint32_t* p, int i0, int n) {
+#pragma unroll
+                    for (int i = 0; i < n; ++i) {
+                        const uint32_t e = 2 * (i0 + i);
+                        const Pair t = fma2(pair(__uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1])), cc, mm);
+                        float x, y;
+                        if (i % 8 == 1 || i % 8 == 4 || i % 8 == 6) {
+                            ex2_poly(t, x, y);
+                        } else {
+                            unpair(t, x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                        }
+                        if (i & 1)
+                            l3 = add2(l3, pair(x, y));
+                        else
+                            l2 = add2(l2, pair(x, y));
+                        p[i] = pack2<BF16>(x, y);
+                    }
+                };
+                // the products of the first 64 keys begin under the last weights
+                uint32_t p[2][32];
+                weights(p[0], 0, 32);
+                tmem_st32(ts, p[0]);
+                weights(p[1], 32, 16);
+                tmem_wait_st();
+                fence_before();
+                mbar_arrive(&p_full[w][0]);
+                weights(p[1] + 16, 48, 16);
+                tmem_st32(ts + 32, p[1]);
+                tmem_wait_st();
+                fence_before();
+                mbar_arrive(&p_full[w][1]);
             }
-            tmem_wait_st();
-            fence_before();
-            mbar_arrive(&p_full[w]);
-        }
-        if (tiles && ok) {
-            if (!mbar_wait_f(&o_full[w], 0, &s_fail, limit)) ok = false;
-            for (uint32_t i = 0; i < tiles - (n0 - 1); ++i)  // long since complete: orders the read of s_foul
-                if (!mbar_wait_f(&v_clean[i], 0, &s_fail, limit)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
-        }
-        if (tiles && ok) {
-            fence_after();
+            if (!ok) break;
+            if (done) ok = __all_sync(0xffffffffu, wait(&o_empty[w], done - 1));  // the last item's sums have been read
             float x0, y0, x1, y1;
             unpair(l2, x0, y0);
             unpair(l3, x1, y1);
-            const float inv = 1.f / ((x0 + y0) + (x1 + y1));
-            const uint32_t at = first_row + w * 128 + row;
-            const bool live = at < len;
-            uint16_t* dst = static_cast<uint16_t*>(a.out) + (long long)(begin + at) * a.out_token + (long long)head * a.out_head;
-#pragma unroll 1
-            for (uint32_t k = 0; k < D; k += 32) {
-                uint32_t o[32];
-                tmem_ld32(o, to + k);
-                tmem_wait_ld();
-                if (s_foul && live) {
-                    // elements that are not finite, of the keys of the last two tiles that this row sees
-                    const uint16_t* v = static_cast<const uint16_t*>(a.v) + (long long)kvh * a.v_head;
-                    for (uint32_t key = first_row; key <= at; ++key) {
-                        const uint16_t* vr = v + (long long)(begin + key) * a.v_token + k;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (k + i < a.hd && not_finite16<BF16>(vr[i]))
-                                o[i] = __float_as_uint(__uint_as_float(o[i]) +
-                                                       (BF16 ? __uint_as_float((uint32_t)vr[i] << 16)
-                                                             : __half2float(__ushort_as_half(vr[i]))));
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i += 8)
-                    if (live && k + i < a.hd) {
-                        uint4 r;
-                        r.x = pack2<BF16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-                        r.y = pack2<BF16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                        r.z = pack2<BF16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-                        r.w = pack2<BF16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-                        *reinterpret_cast<uint4*>(dst + k + i) = r;
-                    }
-            }
+            s_inv[w][row] = 1.f / ((x0 + y0) + (x1 + y1));
+            mbar_arrive(&l_full[w]);
+            ++done;
         }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkRegsRest));
-        // Stage and phase of the i-th tile of the ring: K tile j is 2j, V tile j is 2j + 1.  The V tiles from
-        // n0 - 1 on, whose stages are not used again, land on barriers of their own, for the helpers.
-        auto full_wait = [&](uint32_t i) { return mbar_wait_f(&kv_full[i % kStages], (i / kStages) & 1, &s_fail, limit); };
-        if (warp == 8) {
-            // ---- all products: one thread ------------------------------------------------------------------
-            if (lane == 0) {
-                auto qk = [&](uint32_t w, uint32_t j) {
-                    const uint32_t k = skv + ((2 * j) % kStages) * kTile, q = sq + w * kTile;
-#pragma unroll
-                    for (uint32_t i = 0; i < D / 16; ++i) {
-                        const uint32_t off = (i / 4) * kPkTileBytes + (i % 4) * 32;
-                        mma_ss(tmem + w * 128, desc_k(q + off), desc_k(k + off), idesc<BF16>(128, false), i);
-                    }
-                };
-                auto pv = [&](uint32_t w, uint32_t j) {
-                    const uint32_t v = skv + ((2 * j + 1) % kStages) * kTile;
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        mma_ts(tmem + kTmemO + w * D, tmem + w * 128 + 8 * i, desc_mn(v + i * 2048), idesc<BF16>(D, true), j | i);
-                };
-                bool ok = mbar_wait_f(&q_full, 0, &s_fail, limit) && full_wait(0);
-                uint32_t committed = 0;  // bit w: o_full[w] will be raised
-                if (ok) {
-                    fence_after();
-                    qk(0, 0);
-                    commit(&s_full[0]);
-                    if (n1) {
-                        qk(1, 0);
-                        commit(&s_full[1]);
-                    }
-                    commit(&kv_empty[0]);
-                }
-                for (uint32_t j = 0; j < n && ok; ++j) {
-#pragma unroll
-                    for (uint32_t w = 0; w < 2; ++w) {
-                        const uint32_t mine = w ? n1 : n0;
-                        if (j >= mine || !ok) continue;
-                        const bool last_user = w == 1 || j >= n1, last_k_user = w == 1 || j + 1 >= n1;
-                        ok = mbar_wait_f(&p_full[w], j & 1, &s_fail, limit) &&
-                             (j >= n0 - 1 ? mbar_wait_f(&v_clean[j - (n0 - 1)], 0, &s_fail, limit) : full_wait(2 * j + 1));
-                        if (!ok) break;
-                        fence_after();
-                        pv(w, j);
-                        if (last_user) commit(&kv_empty[(2 * j + 1) % kStages]);
-                        if (j + 1 < mine) {
-                            ok = full_wait(2 * j + 2);
-                            if (!ok) break;
-                            fence_after();
-                            qk(w, j + 1);
-                            commit(&s_full[w]);
-                            if (last_k_user) commit(&kv_empty[(2 * j + 2) % kStages]);
-                        } else {
-                            commit(&o_full[w]);
-                            committed |= 1u << w;
-                        }
-                    }
-                }
-                // every product complete before TMEM and the tiles are released
-                if (!ok) {
-                    commit(&o_full[committed & 1]);  // one more phase of a barrier nobody waits for any more
-                    mbar_drain(&o_full[committed & 1], 0);
-                } else {
-                    mbar_drain(&o_full[0], 0);
-                    if (n1) mbar_drain(&o_full[1], 0);
-                }
-            }
-        } else if (warp == 9) {
-            // ---- loads: one thread -----------------------------------------------------------------------------
-            if (lane == 0) {
-                auto bar_of = [&](uint32_t i) { return i & 1 && i / 2 >= n0 - 1 ? &v_raw[i / 2 - (n0 - 1)] : &kv_full[i % kStages]; };
-                auto load = [&](uint32_t i) {
-                    const CUtensorMap* map = i & 1 ? &vmap : &kmap;
-                    const uint32_t dst = skv + (i % kStages) * kTile;
-                    uint64_t* bar = bar_of(i);
-                    expect_tx(bar, kTile);
-#pragma unroll
-                    for (uint32_t h = 0; h < kHalves; ++h)
-                        tma_tile(dst + h * kPkTileBytes, map, h, kvh, begin + (i / 2) * 128, bar);
-                };
-                const uint32_t q_tiles = n1 ? 2 : 1;
-                expect_tx(&q_full, q_tiles * kTile);
-                for (uint32_t t = 0; t < q_tiles; ++t)
-#pragma unroll
-                    for (uint32_t h = 0; h < kHalves; ++h)
-                        tma_tile(sq + t * kTile + h * kPkTileBytes, &qmap, h, head, begin + first_row + t * 128, &q_full);
-                uint32_t sent = 0;
-                for (uint32_t i = 0; i < 2 * n; ++i) {
-                    if (i >= kStages && !mbar_wait_f(&kv_empty[i % kStages], ((i / kStages) - 1) & 1, &s_fail, limit)) break;
-                    load(i);
-                    sent = i + 1;
-                }
-                mbar_drain(&q_full, 0);
-                for (uint32_t i = sent > kStages ? sent - kStages : 0; i < sent; ++i)
-                    mbar_drain(bar_of(i), i & 1 && i / 2 >= n0 - 1 ? 0 : (i / kStages) & 1);
-            }
-        } else {
-            // ---- V tiles that some row sees only in part: elements that are not finite become 0 ---------------
-            const uint32_t at = tid - 320;
-            for (uint32_t j = n0 - 1; j < n; ++j) {
-                if (!mbar_wait_f(&v_raw[j - (n0 - 1)], 0, &s_fail, limit)) break;
-                const uint32_t v = skv + ((2 * j + 1) % kStages) * kTile;
-                bool foul = false;
-                for (uint32_t i = at; i < kTile / 16; i += 64) {
+    } else if (warp < 12) {
+        // ---- output, and the V tiles that some row sees only in part ------------------------------------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkRegsOut));
+        const uint32_t row = tid & 127, lanes = (32 * (warp & 3)) << 16;
+        uint32_t done[2] = {0, 0}, ring = 0, clean = 0;
+        bool ok = true;
+        Item it;
+        for (uint32_t k = 0; ok && next_item(k, it, false); ++k) {
+            const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1);
+            for (uint32_t j = n0 - 1; j < n && ok; ++j, ++clean) {
+                ok = wait(&v_raw[clean % kPkClean], clean / kPkClean);
+                const uint32_t v = skv + ((ring + 2 * j + 1) % kStages) * kTile;
+                for (uint32_t i = row; i < kTile / 16 && ok; i += 128) {
                     uint32_t x[4];
                     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                                  : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
@@ -554,12 +477,259 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(v + i * 16), "r"(x[0]), "r"(x[1]), "r"(x[2]),
                                      "r"(x[3])
                                      : "memory");
-                        foul = true;
+                        s_foul = k + 1;
                     }
                 }
-                if (foul) s_foul = 1;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&v_clean[j - (n0 - 1)]);
+                mbar_arrive(&v_clean[clean % kPkClean]);
+                ok = ok && wait(&v_clean[clean % kPkClean], clean / kPkClean);  // every thread's part: s_foul is settled
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            const bool foul = ok && *(volatile uint32_t*)&s_foul == k + 1;
+            ring += 2 * n;
+#pragma unroll
+            for (uint32_t w = 0; w < 2; ++w) {
+                if (!ok || (w && !n1)) break;
+                ok = wait(&l_full[w], done[w]) && wait(&o_full[w], done[w]);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ++done[w];
+                fence_after();
+                const float inv = s_inv[w][row];
+                const uint32_t at = it.pair * 256 + w * 128 + row, to = tmem + lanes + kTmemO + w * D;
+                const bool live = at < it.len;
+                uint16_t* dst = static_cast<uint16_t*>(a.out) + (long long)(it.begin + at) * a.out_token + (long long)it.head * a.out_head;
+#pragma unroll 1
+                for (uint32_t d = 0; d < D; d += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(o, to + d);
+                    tmem_wait_ld();
+                    if (foul && live) {
+                        // elements that are not finite, of the keys of the last two tiles that this row sees
+                        const uint16_t* v = static_cast<const uint16_t*>(a.v) + (long long)(it.head / group) * a.v_head;
+                        for (uint32_t key = it.pair * 256; key <= at; ++key) {
+                            const uint16_t* vr = v + (long long)(it.begin + key) * a.v_token + d;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (d + i < a.hd && not_finite16<BF16>(vr[i]))
+                                    o[i] = __float_as_uint(__uint_as_float(o[i]) +
+                                                           (BF16 ? __uint_as_float((uint32_t)vr[i] << 16)
+                                                                 : __half2float(__ushort_as_half(vr[i]))));
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        if (live && d + i < a.hd) {
+                            uint4 r;
+                            r.x = pack2<BF16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+                            r.y = pack2<BF16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                            r.z = pack2<BF16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                            r.w = pack2<BF16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                            *reinterpret_cast<uint4*>(dst + d + i) = r;
+                        }
+                }
+                fence_before();
+                mbar_arrive(&o_empty[w]);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkRegsRest));
+        if (warp == 12 || warp == 15) {
+            // ---- the products of row tile w: one thread ------------------------------------------------------
+            const uint32_t w = warp == 15;
+            if (lane == 0) {
+                uint32_t steps = 0, done = 0, clean = 0, stage = 0, round = 0;  // of the ring's next tile
+                const uint32_t qlo = (sq + w * kTile) >> 4, ts = tmem + w * 128, to = tmem + kTmemO + w * D;
+                auto advance = [&]() {
+                    if (++stage == kStages) {
+                        stage = 0;
+                        ++round;
+                    }
+                };
+                auto full = [&]() { return wait(&kv_full[stage], round); };
+                // S = Q K^T with the ring's next tile, which is then released
+                auto qk = [&]() {
+                    const uint32_t klo = (skv + stage * kTile) >> 4;
+#pragma unroll
+                    for (uint32_t i = 0; i < D / 16; ++i) {
+                        const uint32_t off = ((i / 4) * kPkTileBytes + (i % 4) * 32) >> 4;
+                        mma_ss(ts, desc_k(qlo + off), desc_k(klo + off), idesc<BF16>(128, false), i);
+                    }
+                    commit(&s_full[w]);
+                    commit(&kv_empty[stage]);
+                };
+                bool ok = true;
+                Item it;
+                for (uint32_t k = 0; ok && next_item(k, it, true); ++k) {
+                    const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1), mine = w ? n1 : n0;
+                    if (mine) {
+                        ok = wait(&q_full[w], done) && full();
+                        if (!ok) break;
+                        fence_after();
+                        qk();
+                        if (mine == 1) commit(&q_empty[w]);
+                        advance();
+                    }
+                    for (uint32_t j = 0; j < mine; ++j, ++steps) {
+                        // V tile j, then K tile j + 1 of the ring
+                        const uint32_t vlo = (skv + stage * kTile) >> 4, v_stage = stage;
+                        ok = j >= n0 - 1 ? wait(&v_clean[(clean + j - (n0 - 1)) % kPkClean], (clean + j - (n0 - 1)) / kPkClean) : full();
+                        if (ok && j == 0 && done) ok = wait(&o_empty[w], done - 1);
+                        ok = ok && wait(&p_full[w][0], steps);
+                        if (!ok) break;
+                        fence_after();
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i)
+                            mma_ts(to, ts + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), j | i);
+                        ok = wait(&p_full[w][1], steps);
+                        if (!ok) break;
+                        fence_after();
+#pragma unroll
+                        for (uint32_t i = 4; i < 8; ++i) mma_ts(to, ts + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), 1);
+                        advance();
+                        if (j + 1 < mine) {
+                            ok = full();
+                            if (!ok) break;
+                            fence_after();
+                            qk();
+                            advance();
+                            if (j + 2 == mine) commit(&q_empty[w]);
+                        } else {
+                            commit(&o_full[w]);
+                        }
+                        commit(&kv_empty[v_stage]);
+                    }
+                    if (!ok) break;
+                    done += mine != 0;
+                    // tiles that only the other row tile uses: released once they are there, in the ring's order
+                    for (uint32_t j = 2 * mine; j < 2 * n && ok; ++j) {
+                        ok = full();
+                        if (ok) mbar_arrive(&kv_empty[stage]);
+                        advance();
+                    }
+                    clean += n - (n0 - 1);
+                }
+                // every product complete before TMEM and the tiles are released
+                commit(&drain[w]);
+                mbar_drain(&drain[w], 0);
+            }
+        } else if (warp == 13) {
+            // ---- loads: one thread -----------------------------------------------------------------------------
+            if (lane == 0) {
+                uint32_t ring = 0, clean = 0, sent_q[2] = {0, 0};
+                auto load_q = [&](const Item& it, uint32_t w) {
+                    if (sent_q[w] && !wait(&q_empty[w], sent_q[w] - 1)) return false;
+                    ++sent_q[w];
+                    expect_tx(&q_full[w], kTile);
+#pragma unroll
+                    for (uint32_t h = 0; h < kHalves; ++h)
+                        tma_tile(sq + w * kTile + h * kPkTileBytes, &qmap, h, it.head, it.begin + it.pair * 256 + w * 128, &q_full[w]);
+                    return true;
+                };
+                // tile t of the ring: of K, or of V with a barrier of its own where some row sees it in part
+                auto load_kv = [&](const Item& it, uint32_t t, uint32_t j, const CUtensorMap* map, uint64_t* bar) {
+                    if (t >= kStages && !wait(&kv_empty[t % kStages], t / kStages - 1)) return false;
+                    expect_tx(bar, kTile);
+#pragma unroll
+                    for (uint32_t h = 0; h < kHalves; ++h)
+                        tma_tile(skv + (t % kStages) * kTile + h * kPkTileBytes, map, h, it.head / group, it.begin + j * 128, bar);
+                    return true;
+                };
+                bool ok = true;
+                Item it;
+                for (uint32_t k = 0; ok && next_item(k, it, true); ++k) {
+                    const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1);
+                    ok = load_q(it, 0);
+                    for (uint32_t j = 0; j < n && ok; ++j) {
+                        ok = load_kv(it, ring, j, &kmap, &kv_full[ring % kStages]);
+                        if (!ok) break;
+                        ++ring;
+                        // Q of row tile 1 behind K tile 0: the products wait for that one first
+                        if (j == 0 && n1) ok = load_q(it, 1);
+                        if (!ok) break;
+                        // (a V tile on a barrier of its own keeps its stage's in step with an empty phase)
+                        if (j >= n0 - 1) {
+                            ok = load_kv(it, ring, j, &vmap, &v_raw[clean % kPkClean]);
+                            if (ok) mbar_arrive(&kv_full[ring % kStages]);
+                            clean += ok;
+                        } else {
+                            ok = load_kv(it, ring, j, &vmap, &kv_full[ring % kStages]);
+                        }
+                        ring += ok;
+                    }
+                }
+                // no copy may still be landing when the CTA releases its shared memory: the last of each barrier
+                for (uint32_t w = 0; w < 2; ++w)
+                    if (sent_q[w]) mbar_drain(&q_full[w], (sent_q[w] - 1) & 1);
+                for (uint32_t i = ring > kStages ? ring - kStages : 0; i < ring; ++i) mbar_drain(&kv_full[i % kStages], (i / kStages) & 1);
+                for (uint32_t i = clean > kPkClean ? clean - kPkClean : 0; i < clean; ++i) mbar_drain(&v_raw[i % kPkClean], (i / kPkClean) & 1);
+            }
+        } else if (warp == 14) {
+            // ---- items: pairs of row tiles in descending order, heads innermost -----------------------------------
+            auto tiles_of = [&](uint32_t s, uint32_t* begin, uint32_t* len) -> uint32_t {  // of prompt s, in pairs
+                if (s >= a.seqs) return 0;
+                const uint32_t b = (uint32_t)min(max(a.offsets[s], 0), (int32_t)a.tokens);
+                const uint32_t e = (uint32_t)min(max(a.offsets[s + 1], 0), (int32_t)a.tokens);
+                *begin = b;
+                *len = e > b ? e - b : 0;
+                return (*len + 255) / 256;
+            };
+            uint32_t my_begin = 0, my_len = 0, most = 0, x, y;
+            const uint32_t my_tiles = tiles_of(lane, &my_begin, &my_len);  // the first 32 prompts stay at hand
+            for (uint32_t s = lane; s < a.seqs; s += 32) most = max(most, s < 32 ? my_tiles : tiles_of(s, &x, &y));
+            most = __reduce_max_sync(0xffffffffu, most);
+            // items of one head whose pair number is p or more
+            auto at_least = [&](uint32_t p) {
+                uint32_t sum = my_tiles > p ? my_tiles - p : 0;
+                for (uint32_t s = lane + 32; s < a.seqs; s += 32) {
+                    const uint32_t t = tiles_of(s, &x, &y);
+                    sum += t > p ? t - p : 0;
+                }
+                return __reduce_add_sync(0xffffffffu, sum);
+            };
+            const unsigned long long total = (unsigned long long)at_least(0) * a.heads;
+            for (uint32_t k = 0;; ++k) {
+                const uint32_t c = k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+                const unsigned long long i = (unsigned long long)k * gridDim.x + c;
+                Item it{0, 0, 0, 0};
+                if (i < total) {
+                    const uint32_t t = (uint32_t)(i / a.heads);
+                    it.head = (uint32_t)(i % a.heads);
+                    uint32_t lo = 0, hi = most;  // at_least(lo) > t >= at_least(hi)
+                    uint32_t above = 0;          // at_least(hi)
+                    while (hi - lo > 1) {
+                        const uint32_t mid = (lo + hi) / 2, n = at_least(mid);
+                        if (n > t) {
+                            lo = mid;
+                        } else {
+                            hi = mid;
+                            above = n;
+                        }
+                    }
+                    it.pair = lo;
+                    uint32_t r = t - above;  // the r-th prompt with more than `lo` pairs
+                    for (uint32_t s0 = 0; s0 < a.seqs; s0 += 32) {
+                        uint32_t b = my_begin, l = my_len, n = my_tiles;
+                        if (s0) n = tiles_of(s0 + lane, &b, &l);
+                        const uint32_t has = __ballot_sync(0xffffffffu, n > lo), count = __popc(has);
+                        if (r < count) {
+                            const uint32_t src = __fns(has, 0, r + 1);
+                            it.begin = __shfl_sync(0xffffffffu, b, src);
+                            it.len = __shfl_sync(0xffffffffu, l, src);
+                            break;
+                        }
+                        r -= count;
+                    }
+                }
+                bool ok = true;
+                if (k >= kPkItems) ok = __all_sync(0xffffffffu, wait(&it_empty[k % kPkItems], k / kPkItems - 1));
+                if (!ok) break;
+                if (lane == 0) {
+                    s_item[k % kPkItems] = it;
+                    mbar_arrive(&it_full[k % kPkItems]);
+                }
+                __syncwarp();
+                if (i >= total) break;
             }
         }
         __syncwarp();
@@ -567,7 +737,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 // ---- launches -----------------------------------------------------------------------------------
@@ -620,7 +790,9 @@ static enx_status launch_packed(const CUtensorMap& q, const CUtensorMap& k, cons
                                       (int)PackedShape<D>::kSmem));
         if (dev < kDevices) known[dev].store(1, std::memory_order_release);
     }
-    const dim3 grid(a.tokens / 256 + a.seqs, a.heads);
+    // a CTA per SM, or as many as there can be items
+    const uint64_t most = ((uint64_t)a.tokens / 256 + a.seqs) * a.heads;
+    const uint32_t grid = (uint32_t)(most < 148 ? most : 148);
     k_attn_packed<D, BF16><<<grid, kPkThreads, PackedShape<D>::kSmem, st>>>(q, k, v, a);
     ENX_CUDA(cudaGetLastError());
     return ENX_OK;

@@ -2,8 +2,8 @@
 
 Bound: scores are f32 sums of hd products of 16-bit values, exact products, each of hd/16 + 1
 accumulations cut at 2^-22 of the largest partial sum, at most Q = scale * sum |q k|: 2^-18 Q with
-hd 128; a weight is off by a factor exp(2 * 2^-18 Q) and by 2^-20 (exp2, sums, quotient), and its rounding
-to 16 bits is half a step (weights below f16's normal numbers: 2^-25 of the largest, times the keys).
+hd 128; a weight is off by a factor exp(2 * 2^-18 Q) and by 7.6e-5 (the cubic of some exponentials, 7.5e-5,
+and f32 roundings), which acts above and below the quotient, and its rounding to 16 bits is half a step (weights below f16's normal numbers: 2^-25 of the largest, times the keys).
 Outputs are rounded once more, half a step."""
 
 import math
@@ -45,7 +45,7 @@ def reference(q, k, v, scale):
         p = torch.softmax(s, -1)
         big = ((qq.abs() @ kk.abs().T) * scale).masked_fill(~seen, 0).amax(-1, keepdim=True)
         outs.append(p @ vv)
-        rel = 2 * torch.expm1(2.0 ** -17 * big) + 2.0 ** -20 + half
+        rel = 2 * torch.expm1(2.0 ** -17 * big) + 2 * 7.6e-5 + half
         tiny = p.amax(-1, keepdim=True) * 2.0 ** -25 * (seen.double() @ vv.abs())
         bounds.append(rel * (p @ vv.abs()) + tiny)
     return torch.stack(outs, 1), torch.stack(bounds, 1)

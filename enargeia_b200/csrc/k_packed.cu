@@ -26,11 +26,11 @@
 // shares even without a counter.
 //
 // Warp roles, synchronised by mbarriers with bounded waits:
-//   warps 0-3, 4-7  softmax of row tile 0 and 1 (thread = row)
-//   warps 8-11      output of both row tiles; and the V tiles that some row sees only in part (below)
-//   warps 12, 15    lane 0 issues the products of row tile 0 and 1 (and warp 12 owns TMEM)
-//   warp 13         lane 0 loads Q, K and V tiles by TMA (128-byte swizzle; 64-element halves of a row)
-//   warp 14         finds the items
+//   warps 0, 3      lane 0 issues the products of row tile 0 and 1 (and warp 0 owns TMEM)
+//   warp 1          lane 0 loads Q, K and V tiles by TMA (128-byte swizzle; 64-element halves of a row)
+//   warp 2          finds the items
+//   warps 4-7, 8-11 softmax of row tile 0 and 1 (thread = row)
+//   warps 12-15     output of both row tiles; and the V tiles that some row sees only in part (below)
 //
 // A weight of zero times a V element that is not finite would be NaN.  The last two key tiles of an item
 // are the only ones that hold keys which some row does not see, so in those the output warps replace
@@ -67,6 +67,12 @@ struct PackedShape {
     static constexpr uint32_t kTile = kHalves * kPkTileBytes;        // a Q, K or V tile
     static constexpr uint32_t kStages = D == 64 ? 6 : 4;             // of K and V tiles, alternating
     static constexpr uint32_t kSmem = (2 + kStages) * kTile + 1024;  // and room to align
+    // TMEM columns of row tile w: S, P and O.  At hd 64 P has columns of its own, and the next scores are
+    // multiplied while the present ones become weights; at hd 128 there is room only over S.
+    static constexpr bool kApart = D == 64;
+    static constexpr uint32_t s_col(uint32_t w) { return kApart ? w * 256 : w * 128; }
+    static constexpr uint32_t p_col(uint32_t w) { return kApart ? w * 256 + 128 : w * 128; }
+    static constexpr uint32_t o_col(uint32_t w) { return kApart ? w * 256 + 192 : 256 + w * 128; }
 };
 
 struct PackedArgs {
@@ -265,10 +271,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                   const __grid_constant__ CUtensorMap vmap, PackedArgs a) {
     using Sh = PackedShape<D>;
     constexpr uint32_t kStages = Sh::kStages, kTile = Sh::kTile, kHalves = Sh::kHalves;
-    constexpr uint32_t kTmemO = 256;  // columns: S (and P) of the two row tiles, then O of each
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t kv_full[kStages], kv_empty[kStages], v_raw[kPkClean], v_clean[kPkClean];
-    __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], l_full[2], o_empty[2], drain[2];
+    __shared__ __align__(8) uint64_t q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], l_full[2], o_empty[2], drain[2], lead;
+    __shared__ __align__(8) uint64_t s_free[2], pv_done[2];  // S is in registers; P may be overwritten (kApart)
     __shared__ __align__(8) uint64_t it_full[kPkItems], it_empty[kPkItems];
     __shared__ Item s_item[kPkItems];
     __shared__ float s_inv[2][128];
@@ -295,6 +301,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             init(&it_full[i], 1);
             init(&it_empty[i], 15);  // 8 softmax warps, 4 output warps, 2 of products, loads
         }
+        init(&lead, 128);
         for (int i = 0; i < 2; ++i) {
             init(&q_full[i], 1);
             init(&q_empty[i], 1);
@@ -305,10 +312,12 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             init(&l_full[i], 128);
             init(&o_empty[i], 128);
             init(&drain[i], 1);
+            init(&s_free[i], 128);
+            init(&pv_done[i], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&tmem_base)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -334,12 +343,12 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     auto tiles0 = [](const Item& it) { return 2 * it.pair + 1; };
     auto tiles1 = [](const Item& it) { return it.pair * 256 + 128 < it.len ? 2 * it.pair + 2 : 0; };
 
-    if (warp < 8) {
+    if (warp >= 4 && warp < 12) {
         // ---- softmax of row tile w: thread = row ---------------------------------------------------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPkRegsSoftmax));
-        const uint32_t w = warp >> 2, row = tid & 127;
+        const uint32_t w = (warp >> 2) - 1, row = tid & 127;
         const uint32_t lanes = (32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + w * 128, to = tmem + lanes + kTmemO + w * D;
+        const uint32_t ts = tmem + lanes + Sh::s_col(w), tp = tmem + lanes + Sh::p_col(w), to = tmem + lanes + Sh::o_col(w);
         const float c = a.scale_log2;
         uint32_t steps = 0, done = 0;  // key tiles and items of this row tile so far
         bool ok = true;
@@ -357,6 +366,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) tmem_ld32(s[i], ts + 32 * i);
                 tmem_wait_ld();
+                if (Sh::kApart) {
+                    fence_before();
+                    mbar_arrive(&s_free[w]);
+                }
                 if (j + 1 == tiles) {  // the diagonal: key column > row is not seen
 #pragma unroll
                     for (int i = 0; i < 128; ++i)
@@ -386,7 +399,12 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     l2 = pair(x * f, y * f);
                     unpair(l3, x, y);
                     l3 = pair(x * f, y * f);
-                    // the product of the last key tile is complete: this tile's scores were issued after it
+                    // (hd 128: the last key tile's product is complete, as these scores were issued after it)
+                    if (Sh::kApart) {
+                        ok = __all_sync(0xffffffffu, wait(&pv_done[w], steps - 1));
+                        if (!ok) break;
+                        fence_after();
+                    }
 #pragma unroll 1
                     for (uint32_t d = 0; d < D; d += 32) {
                         uint32_t o[32];
@@ -423,16 +441,22 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 // the products of the first 64 keys begin under the last weights
                 uint32_t p[2][32];
                 weights(p[0], 0, 32);
-                tmem_st32(ts, p[0]);
+                if (Sh::kApart && steps) {  // the last weights have been used
+                    ok = __all_sync(0xffffffffu, wait(&pv_done[w], steps - 1));
+                    if (!ok) break;
+                    fence_after();
+                }
+                tmem_st32(tp, p[0]);
                 weights(p[1], 32, 16);
                 tmem_wait_st();
                 fence_before();
                 mbar_arrive(&p_full[w][0]);
                 weights(p[1] + 16, 48, 16);
-                tmem_st32(ts + 32, p[1]);
+                tmem_st32(tp + 32, p[1]);
                 tmem_wait_st();
                 fence_before();
                 mbar_arrive(&p_full[w][1]);
+                if (w == 0 && j == 0 && tiles1(it)) mbar_arrive(&lead);
             }
             if (!ok) break;
             if (done) ok = __all_sync(0xffffffffu, wait(&o_empty[w], done - 1));  // the last item's sums have been read
@@ -443,7 +467,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
             mbar_arrive(&l_full[w]);
             ++done;
         }
-    } else if (warp < 12) {
+    } else if (warp >= 12) {
         // ---- output, and the V tiles that some row sees only in part ------------------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkRegsOut));
         const uint32_t row = tid & 127, lanes = (32 * (warp & 3)) << 16;
@@ -496,7 +520,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 ++done[w];
                 fence_after();
                 const float inv = s_inv[w][row];
-                const uint32_t at = it.pair * 256 + w * 128 + row, to = tmem + lanes + kTmemO + w * D;
+                const uint32_t at = it.pair * 256 + w * 128 + row, to = tmem + lanes + Sh::o_col(w);
                 const bool live = at < it.len;
                 uint16_t* dst = static_cast<uint16_t*>(a.out) + (long long)(it.begin + at) * a.out_token + (long long)it.head * a.out_head;
 #pragma unroll 1
@@ -534,12 +558,15 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkRegsRest));
-        if (warp == 12 || warp == 15) {
+        if (warp == 0 || warp == 3) {
             // ---- the products of row tile w: one thread ------------------------------------------------------
-            const uint32_t w = warp == 15;
+            const uint32_t w = warp == 3;
             if (lane == 0) {
-                uint32_t steps = 0, done = 0, clean = 0, stage = 0, round = 0;  // of the ring's next tile
-                const uint32_t qlo = (sq + w * kTile) >> 4, ts = tmem + w * 128, to = tmem + kTmemO + w * D;
+                uint32_t steps = 0, done = 0, clean = 0;
+                uint32_t stage = 0, round = 0;  // of the ring's next tile
+                uint32_t scores = 0;            // products Q K^T so far
+                const uint32_t qlo = (sq + w * kTile) >> 4;
+                const uint32_t ts = tmem + Sh::s_col(w), tp = tmem + Sh::p_col(w), to = tmem + Sh::o_col(w);
                 auto advance = [&]() {
                     if (++stage == kStages) {
                         stage = 0;
@@ -547,8 +574,11 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     }
                 };
                 auto full = [&]() { return wait(&kv_full[stage], round); };
-                // S = Q K^T with the ring's next tile, which is then released
-                auto qk = [&]() {
+                // S = Q K^T with the ring's next tile, which is there and then released
+                auto qk = [&](bool last) {
+                    if (Sh::kApart && scores && !wait(&s_free[w], scores - 1)) return false;
+                    ++scores;
+                    fence_after();
                     const uint32_t klo = (skv + stage * kTile) >> 4;
 #pragma unroll
                     for (uint32_t i = 0; i < D / 16; ++i) {
@@ -557,6 +587,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     }
                     commit(&s_full[w]);
                     commit(&kv_empty[stage]);
+                    if (last) commit(&q_empty[w]);
+                    advance();
+                    return true;
                 };
                 bool ok = true;
                 Item it;
@@ -564,39 +597,37 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1), mine = w ? n1 : n0;
                     if (mine) {
                         ok = wait(&q_full[w], done) && full();
+                        // Row tile 1 sets out when tile 0's first weights are done: in step, the two would
+                        // want the same pipes at the same time and leave them idle together.
+                        if (ok && w) ok = wait(&lead, done);
+                        ok = ok && qk(mine == 1);
                         if (!ok) break;
-                        fence_after();
-                        qk();
-                        if (mine == 1) commit(&q_empty[w]);
-                        advance();
                     }
                     for (uint32_t j = 0; j < mine; ++j, ++steps) {
-                        // V tile j, then K tile j + 1 of the ring
+                        // V tile j, then K tile j + 1 of the ring; what is there early is waited for early
                         const uint32_t vlo = (skv + stage * kTile) >> 4, v_stage = stage;
+                        const bool more = j + 1 < mine;
                         ok = j >= n0 - 1 ? wait(&v_clean[(clean + j - (n0 - 1)) % kPkClean], (clean + j - (n0 - 1)) / kPkClean) : full();
+                        advance();
+                        ok = ok && (!more || full());
+                        if (Sh::kApart && more) ok = ok && qk(j + 2 == mine);
                         if (ok && j == 0 && done) ok = wait(&o_empty[w], done - 1);
                         ok = ok && wait(&p_full[w][0], steps);
                         if (!ok) break;
                         fence_after();
 #pragma unroll
                         for (uint32_t i = 0; i < 4; ++i)
-                            mma_ts(to, ts + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), j | i);
+                            mma_ts(to, tp + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), j | i);
                         ok = wait(&p_full[w][1], steps);
                         if (!ok) break;
                         fence_after();
 #pragma unroll
-                        for (uint32_t i = 4; i < 8; ++i) mma_ts(to, ts + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), 1);
-                        advance();
-                        if (j + 1 < mine) {
-                            ok = full();
-                            if (!ok) break;
-                            fence_after();
-                            qk();
-                            advance();
-                            if (j + 2 == mine) commit(&q_empty[w]);
-                        } else {
-                            commit(&o_full[w]);
-                        }
+                        for (uint32_t i = 4; i < 8; ++i) mma_ts(to, tp + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), 1);
+                        if (Sh::kApart)
+                            commit(&pv_done[w]);
+                        else if (more)
+                            ok = qk(j + 2 == mine);
+                        if (!more) commit(&o_full[w]);
                         commit(&kv_empty[v_stage]);
                     }
                     if (!ok) break;
@@ -613,7 +644,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 commit(&drain[w]);
                 mbar_drain(&drain[w], 0);
             }
-        } else if (warp == 13) {
+        } else if (warp == 1) {
             // ---- loads: one thread -----------------------------------------------------------------------------
             if (lane == 0) {
                 uint32_t ring = 0, clean = 0, sent_q[2] = {0, 0};
@@ -664,7 +695,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 for (uint32_t i = ring > kStages ? ring - kStages : 0; i < ring; ++i) mbar_drain(&kv_full[i % kStages], (i / kStages) & 1);
                 for (uint32_t i = clean > kPkClean ? clean - kPkClean : 0; i < clean; ++i) mbar_drain(&v_raw[i % kPkClean], (i / kPkClean) & 1);
             }
-        } else if (warp == 14) {
+        } else {
             // ---- items: pairs of row tiles in descending order, heads innermost -----------------------------------
             auto tiles_of = [&](uint32_t s, uint32_t* begin, uint32_t* len) -> uint32_t {  // of prompt s, in pairs
                 if (s >= a.seqs) return 0;
@@ -737,7 +768,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
 // ---- launches -----------------------------------------------------------------------------------

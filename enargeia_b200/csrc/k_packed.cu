@@ -26,7 +26,8 @@
 // shares even without a counter.
 //
 // Warp roles, synchronised by mbarriers with bounded waits:
-//   warps 0, 3      lane 0 issues the products of row tile 0 and 1 (and warp 0 owns TMEM)
+//   warps 0, 3      lane 0 issues products: hd 64, scores and outputs, hd 128, row tile 0 and 1 (and warp 0
+//                   owns TMEM).  A wait or a commit costs that thread 150 clocks or more, so they are few.
 //   warp 1          lane 0 loads Q, K and V tiles by TMA (128-byte swizzle; 64-element halves of a row)
 //   warp 2          finds the items
 //   warps 4-7, 8-11 softmax of row tile 0 and 1 (thread = row)
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         };
         for (uint32_t i = 0; i < kStages; ++i) {
             init(&kv_full[i], 1);
-            init(&kv_empty[i], 2);  // both row tiles
+            init(&kv_empty[i], Sh::kApart ? 1 : 2);  // one thread's release, or both row tiles'
         }
         for (uint32_t i = 0; i < kPkClean; ++i) {
             init(&v_raw[i], 1);
@@ -438,7 +439,6 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         p[i] = pack2<BF16>(x, y);
                     }
                 };
-                // the products of the first 64 keys begin under the last weights
                 uint32_t p[2][32];
                 weights(p[0], 0, 32);
                 if (Sh::kApart && steps) {  // the last weights have been used
@@ -447,16 +447,20 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     fence_after();
                 }
                 tmem_st32(tp, p[0]);
-                weights(p[1], 32, 16);
-                tmem_wait_st();
-                fence_before();
-                mbar_arrive(&p_full[w][0]);
-                weights(p[1] + 16, 48, 16);
+                if (Sh::kApart) {
+                    weights(p[1], 32, 32);
+                } else {  // the products of the first 64 keys begin under the last weights
+                    weights(p[1], 32, 16);
+                    tmem_wait_st();
+                    fence_before();
+                    mbar_arrive(&p_full[w][0]);
+                    weights(p[1] + 16, 48, 16);
+                }
                 tmem_st32(tp + 32, p[1]);
                 tmem_wait_st();
                 fence_before();
                 mbar_arrive(&p_full[w][1]);
-                if (w == 0 && j == 0 && tiles1(it)) mbar_arrive(&lead);
+                if (!Sh::kApart && w == 0 && j == 0 && tiles1(it)) mbar_arrive(&lead);
             }
             if (!ok) break;
             if (done) ok = __all_sync(0xffffffffu, wait(&o_empty[w], done - 1));  // the last item's sums have been read
@@ -558,13 +562,98 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkRegsRest));
-        if (warp == 0 || warp == 3) {
+        if (Sh::kApart && warp == 0) {
+            // ---- scores of both row tiles: one thread; it is ahead of the softmax by a key tile ------------------
+            if (lane == 0) {
+                uint32_t scores[2] = {0, 0}, done[2] = {0, 0}, stage = 0, round = 0;  // of the ring's next K tile
+                bool ok = true;
+                Item it;
+                for (uint32_t k = 0; ok && next_item(k, it, true); ++k) {
+                    const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1);
+                    for (uint32_t j = 0; j < n && ok; ++j) {
+                        const uint32_t klo = (skv + stage * kTile) >> 4;
+                        ok = wait(&kv_full[stage], round);
+#pragma unroll
+                        for (uint32_t w = 0; w < 2; ++w) {
+                            const uint32_t mine = w ? n1 : n0, qlo = (sq + w * kTile) >> 4;
+                            if (!ok || j >= mine) continue;
+                            if (j == 0) ok = wait(&q_full[w], done[w]);
+                            if (ok && scores[w]) ok = wait(&s_free[w], scores[w] - 1);
+                            if (!ok) break;
+                            ++scores[w];
+                            fence_after();
+#pragma unroll
+                            for (uint32_t i = 0; i < D / 16; ++i)
+                                mma_ss(tmem + Sh::s_col(w), desc_k(qlo + 2 * i), desc_k(klo + 2 * i), idesc<BF16>(128, false), i);
+                            commit(&s_full[w]);
+                            if (j + 1 == mine) {
+                                commit(&q_empty[w]);
+                                ++done[w];
+                            }
+                        }
+                        commit(&kv_empty[stage]);
+                        stage += 2;
+                        if (stage == kStages) {
+                            stage = 0;
+                            ++round;
+                        }
+                    }
+                }
+                commit(&drain[0]);
+                mbar_drain(&drain[0], 0);
+            }
+        } else if (Sh::kApart && warp == 3) {
+            // ---- weights times V, of both row tiles: one thread ----------------------------------------------------
+            if (lane == 0) {
+                uint32_t steps[2] = {0, 0}, done[2] = {0, 0}, clean = 0, stage = 1, round = 0;  // of the ring's next V tile
+                bool ok = true;
+                Item it;
+                for (uint32_t k = 0; ok && next_item(k, it, true); ++k) {
+                    const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1);
+                    for (uint32_t j = 0; j < n && ok; ++j) {
+                        const uint32_t vlo = (skv + stage * kTile) >> 4;
+                        if (j >= n0 - 1) {
+                            ok = wait(&v_clean[clean % kPkClean], clean / kPkClean);
+                            ++clean;
+                        } else {
+                            ok = wait(&kv_full[stage], round);
+                        }
+#pragma unroll
+                        for (uint32_t w = 0; w < 2; ++w) {
+                            const uint32_t mine = w ? n1 : n0;
+                            if (!ok || j >= mine) continue;
+                            if (j == 0 && done[w]) ok = wait(&o_empty[w], done[w] - 1);
+                            ok = ok && wait(&p_full[w][1], steps[w]);
+                            if (!ok) break;
+                            ++steps[w];
+                            fence_after();
+#pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i)
+                                mma_ts(tmem + Sh::o_col(w), tmem + Sh::p_col(w) + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), j | i);
+                            commit(&pv_done[w]);
+                            if (j + 1 == mine) {
+                                commit(&o_full[w]);
+                                ++done[w];
+                            }
+                        }
+                        commit(&kv_empty[stage]);
+                        stage += 2;
+                        if (stage > kStages) {
+                            stage = 1;
+                            ++round;
+                        }
+                    }
+                }
+                // every product complete before TMEM and the tiles are released
+                commit(&drain[1]);
+                mbar_drain(&drain[1], 0);
+            }
+        } else if (warp == 0 || warp == 3) {
             // ---- the products of row tile w: one thread ------------------------------------------------------
             const uint32_t w = warp == 3;
             if (lane == 0) {
                 uint32_t steps = 0, done = 0, clean = 0;
                 uint32_t stage = 0, round = 0;  // of the ring's next tile
-                uint32_t scores = 0;            // products Q K^T so far
                 const uint32_t qlo = (sq + w * kTile) >> 4;
                 const uint32_t ts = tmem + Sh::s_col(w), tp = tmem + Sh::p_col(w), to = tmem + Sh::o_col(w);
                 auto advance = [&]() {
@@ -576,9 +665,6 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 auto full = [&]() { return wait(&kv_full[stage], round); };
                 // S = Q K^T with the ring's next tile, which is there and then released
                 auto qk = [&](bool last) {
-                    if (Sh::kApart && scores && !wait(&s_free[w], scores - 1)) return false;
-                    ++scores;
-                    fence_after();
                     const uint32_t klo = (skv + stage * kTile) >> 4;
 #pragma unroll
                     for (uint32_t i = 0; i < D / 16; ++i) {
@@ -589,7 +675,6 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     commit(&kv_empty[stage]);
                     if (last) commit(&q_empty[w]);
                     advance();
-                    return true;
                 };
                 bool ok = true;
                 Item it;
@@ -600,8 +685,9 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         // Row tile 1 sets out when tile 0's first weights are done: in step, the two would
                         // want the same pipes at the same time and leave them idle together.
                         if (ok && w) ok = wait(&lead, done);
-                        ok = ok && qk(mine == 1);
                         if (!ok) break;
+                        fence_after();
+                        qk(mine == 1);
                     }
                     for (uint32_t j = 0; j < mine; ++j, ++steps) {
                         // V tile j, then K tile j + 1 of the ring; what is there early is waited for early
@@ -610,7 +696,6 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         ok = j >= n0 - 1 ? wait(&v_clean[(clean + j - (n0 - 1)) % kPkClean], (clean + j - (n0 - 1)) / kPkClean) : full();
                         advance();
                         ok = ok && (!more || full());
-                        if (Sh::kApart && more) ok = ok && qk(j + 2 == mine);
                         if (ok && j == 0 && done) ok = wait(&o_empty[w], done - 1);
                         ok = ok && wait(&p_full[w][0], steps);
                         if (!ok) break;
@@ -623,11 +708,10 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         fence_after();
 #pragma unroll
                         for (uint32_t i = 4; i < 8; ++i) mma_ts(to, tp + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), 1);
-                        if (Sh::kApart)
-                            commit(&pv_done[w]);
-                        else if (more)
-                            ok = qk(j + 2 == mine);
-                        if (!more) commit(&o_full[w]);
+                        if (more)
+                            qk(j + 2 == mine);
+                        else
+                            commit(&o_full[w]);
                         commit(&kv_empty[v_stage]);
                     }
                     if (!ok) break;

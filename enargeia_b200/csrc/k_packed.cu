@@ -26,8 +26,8 @@
 // shares even without a counter.
 //
 // Warp roles, synchronised by mbarriers with bounded waits:
-//   warps 0, 3      lane 0 issues products: hd 64, scores and outputs, hd 128, row tile 0 and 1 (and warp 0
-//                   owns TMEM).  A wait or a commit costs that thread 150 clocks or more, so they are few.
+//   warps 0, 3      issue the products: hd 64, scores and outputs, hd 128, row tile 0 and 1 (and warp 0
+//                   owns TMEM)
 //   warp 1          lane 0 loads Q, K and V tiles by TMA (128-byte swizzle; 64-element halves of a row)
 //   warp 2          finds the items
 //   warps 4-7, 8-11 softmax of row tile 0 and 1 (thread = row)
@@ -120,6 +120,13 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 
 __device__ __forceinline__ void commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar)) : "memory");
+}
+
+// One lane of the (converged) warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
 }
 
 // Shared-memory matrix descriptors of tiles written by TMA with the 128-byte swizzle: rows of 128
@@ -562,110 +569,122 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPkRegsRest));
+        // The product warps run their loops as a whole, on values that the compiler sees to be the same in all
+        // lanes (votes, shuffles from lane 0), so that descriptors stay in uniform registers; one elected
+        // lane issues.  A tcgen05 operand that comes from one lane's own register costs some 15 clocks.
+        const bool lead_lane = elect_one();
+        auto wait_all = [&](uint64_t* bar, uint32_t phase) { return (bool)__all_sync(0xffffffffu, wait(bar, phase)); };
+        auto next_all = [&](uint32_t k, uint32_t* n0, uint32_t* n1) {  // the key tiles of the k-th item's row tiles
+            Item it{};
+            const bool got = next_item(k, it, false);
+            *n0 = __shfl_sync(0xffffffffu, got ? tiles0(it) : 0u, 0);
+            *n1 = __shfl_sync(0xffffffffu, got ? tiles1(it) : 0u, 0);
+            return *n0 != 0;
+        };
         if (Sh::kApart && warp == 0) {
-            // ---- scores of both row tiles: one thread; it is ahead of the softmax by a key tile ------------------
-            if (lane == 0) {
-                uint32_t scores[2] = {0, 0}, done[2] = {0, 0}, stage = 0, round = 0;  // of the ring's next K tile
-                bool ok = true;
-                Item it;
-                for (uint32_t k = 0; ok && next_item(k, it, true); ++k) {
-                    const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1);
-                    for (uint32_t j = 0; j < n && ok; ++j) {
-                        const uint32_t klo = (skv + stage * kTile) >> 4;
-                        ok = wait(&kv_full[stage], round);
+            // ---- scores of both row tiles, ahead of the softmax by a key tile ------------------------------------
+            uint32_t scores[2] = {0, 0}, done[2] = {0, 0}, stage = 0, round = 0;  // of the ring's next K tile
+            bool ok = true;
+            uint32_t n0, n1;
+            for (uint32_t k = 0; ok && next_all(k, &n0, &n1); ++k) {
+                const uint32_t n = max(n0, n1);
+                for (uint32_t j = 0; j < n && ok; ++j) {
+                    const uint32_t klo = (skv + stage * kTile) >> 4;
+                    ok = wait_all(&kv_full[stage], round);
 #pragma unroll
-                        for (uint32_t w = 0; w < 2; ++w) {
-                            const uint32_t mine = w ? n1 : n0, qlo = (sq + w * kTile) >> 4;
-                            if (!ok || j >= mine) continue;
-                            if (j == 0) ok = wait(&q_full[w], done[w]);
-                            if (ok && scores[w]) ok = wait(&s_free[w], scores[w] - 1);
-                            if (!ok) break;
-                            ++scores[w];
-                            fence_after();
+                    for (uint32_t w = 0; w < 2; ++w) {
+                        const uint32_t mine = w ? n1 : n0, qlo = (sq + w * kTile) >> 4;
+                        if (!ok || j >= mine) continue;
+                        if (j == 0) ok = wait_all(&q_full[w], done[w]);
+                        if (ok && scores[w]) ok = wait_all(&s_free[w], scores[w] - 1);
+                        if (!ok) break;
+                        ++scores[w];
+                        fence_after();
+                        if (lead_lane) {
 #pragma unroll
                             for (uint32_t i = 0; i < D / 16; ++i)
                                 mma_ss(tmem + Sh::s_col(w), desc_k(qlo + 2 * i), desc_k(klo + 2 * i), idesc<BF16>(128, false), i);
                             commit(&s_full[w]);
-                            if (j + 1 == mine) {
-                                commit(&q_empty[w]);
-                                ++done[w];
-                            }
+                            if (j + 1 == mine) commit(&q_empty[w]);
                         }
-                        commit(&kv_empty[stage]);
-                        stage += 2;
-                        if (stage == kStages) {
-                            stage = 0;
-                            ++round;
-                        }
+                        done[w] += j + 1 == mine;
+                    }
+                    if (lead_lane) commit(&kv_empty[stage]);
+                    stage += 2;
+                    if (stage == kStages) {
+                        stage = 0;
+                        ++round;
                     }
                 }
+            }
+            if (lead_lane) {
                 commit(&drain[0]);
                 mbar_drain(&drain[0], 0);
             }
         } else if (Sh::kApart && warp == 3) {
-            // ---- weights times V, of both row tiles: one thread ----------------------------------------------------
-            if (lane == 0) {
-                uint32_t steps[2] = {0, 0}, done[2] = {0, 0}, clean = 0, stage = 1, round = 0;  // of the ring's next V tile
-                bool ok = true;
-                Item it;
-                for (uint32_t k = 0; ok && next_item(k, it, true); ++k) {
-                    const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1);
-                    for (uint32_t j = 0; j < n && ok; ++j) {
-                        const uint32_t vlo = (skv + stage * kTile) >> 4;
-                        if (j >= n0 - 1) {
-                            ok = wait(&v_clean[clean % kPkClean], clean / kPkClean);
-                            ++clean;
-                        } else {
-                            ok = wait(&kv_full[stage], round);
-                        }
+            // ---- weights times V, of both row tiles ------------------------------------------------------------------
+            uint32_t steps[2] = {0, 0}, done[2] = {0, 0}, clean = 0, stage = 1, round = 0;  // of the ring's next V tile
+            bool ok = true;
+            uint32_t n0, n1;
+            for (uint32_t k = 0; ok && next_all(k, &n0, &n1); ++k) {
+                const uint32_t n = max(n0, n1);
+                for (uint32_t j = 0; j < n && ok; ++j) {
+                    const uint32_t vlo = (skv + stage * kTile) >> 4;
+                    if (j >= n0 - 1) {
+                        ok = wait_all(&v_clean[clean % kPkClean], clean / kPkClean);
+                        ++clean;
+                    } else {
+                        ok = wait_all(&kv_full[stage], round);
+                    }
 #pragma unroll
-                        for (uint32_t w = 0; w < 2; ++w) {
-                            const uint32_t mine = w ? n1 : n0;
-                            if (!ok || j >= mine) continue;
-                            if (j == 0 && done[w]) ok = wait(&o_empty[w], done[w] - 1);
-                            ok = ok && wait(&p_full[w][1], steps[w]);
-                            if (!ok) break;
-                            ++steps[w];
-                            fence_after();
+                    for (uint32_t w = 0; w < 2; ++w) {
+                        const uint32_t mine = w ? n1 : n0;
+                        if (!ok || j >= mine) continue;
+                        if (j == 0 && done[w]) ok = wait_all(&o_empty[w], done[w] - 1);
+                        ok = ok && wait_all(&p_full[w][1], steps[w]);
+                        if (!ok) break;
+                        ++steps[w];
+                        fence_after();
+                        if (lead_lane) {
 #pragma unroll
                             for (uint32_t i = 0; i < 8; ++i)
                                 mma_ts(tmem + Sh::o_col(w), tmem + Sh::p_col(w) + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), j | i);
                             commit(&pv_done[w]);
-                            if (j + 1 == mine) {
-                                commit(&o_full[w]);
-                                ++done[w];
-                            }
+                            if (j + 1 == mine) commit(&o_full[w]);
                         }
-                        commit(&kv_empty[stage]);
-                        stage += 2;
-                        if (stage > kStages) {
-                            stage = 1;
-                            ++round;
-                        }
+                        done[w] += j + 1 == mine;
+                    }
+                    if (lead_lane) commit(&kv_empty[stage]);
+                    stage += 2;
+                    if (stage > kStages) {
+                        stage = 1;
+                        ++round;
                     }
                 }
-                // every product complete before TMEM and the tiles are released
+            }
+            // every product complete before TMEM and the tiles are released
+            if (lead_lane) {
                 commit(&drain[1]);
                 mbar_drain(&drain[1], 0);
             }
         } else if (warp == 0 || warp == 3) {
-            // ---- the products of row tile w: one thread ------------------------------------------------------
-            const uint32_t w = warp == 3;
-            if (lane == 0) {
-                uint32_t steps = 0, done = 0, clean = 0;
-                uint32_t stage = 0, round = 0;  // of the ring's next tile
-                const uint32_t qlo = (sq + w * kTile) >> 4;
-                const uint32_t ts = tmem + Sh::s_col(w), tp = tmem + Sh::p_col(w), to = tmem + Sh::o_col(w);
-                auto advance = [&]() {
-                    if (++stage == kStages) {
-                        stage = 0;
-                        ++round;
-                    }
-                };
-                auto full = [&]() { return wait(&kv_full[stage], round); };
-                // S = Q K^T with the ring's next tile, which is there and then released
-                auto qk = [&](bool last) {
-                    const uint32_t klo = (skv + stage * kTile) >> 4;
+            // ---- the products of row tile w ------------------------------------------------------------------------------
+            const uint32_t w = __shfl_sync(0xffffffffu, warp == 3 ? 1u : 0u, 0);
+            uint32_t steps = 0, done = 0, clean = 0;
+            uint32_t stage = 0, round = 0;  // of the ring's next tile
+            const uint32_t qlo = (sq + w * kTile) >> 4;
+            const uint32_t ts = tmem + Sh::s_col(w), tp = tmem + Sh::p_col(w), to = tmem + Sh::o_col(w);
+            auto advance = [&]() {
+                if (++stage == kStages) {
+                    stage = 0;
+                    ++round;
+                }
+            };
+            auto full = [&]() { return wait_all(&kv_full[stage], round); };
+            // S = Q K^T with the ring's next tile, which is there and then released
+            auto qk = [&](bool last) {
+                const uint32_t klo = (skv + stage * kTile) >> 4;
+                if (lead_lane) {
 #pragma unroll
                     for (uint32_t i = 0; i < D / 16; ++i) {
                         const uint32_t off = ((i / 4) * kPkTileBytes + (i % 4) * 32) >> 4;
@@ -674,57 +693,62 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     commit(&s_full[w]);
                     commit(&kv_empty[stage]);
                     if (last) commit(&q_empty[w]);
+                }
+                advance();
+            };
+            bool ok = true;
+            uint32_t n0, n1;
+            for (uint32_t k = 0; ok && next_all(k, &n0, &n1); ++k) {
+                const uint32_t n = max(n0, n1), mine = w ? n1 : n0;
+                if (mine) {
+                    ok = wait_all(&q_full[w], done) && full();
+                    // Row tile 1 sets out when tile 0's first weights are done: in step, the two would
+                    // want the same pipes at the same time and leave them idle together.
+                    if (ok && w) ok = wait_all(&lead, done);
+                    if (!ok) break;
+                    fence_after();
+                    qk(mine == 1);
+                }
+                for (uint32_t j = 0; j < mine; ++j, ++steps) {
+                    // V tile j, then K tile j + 1 of the ring; what is there early is waited for early
+                    const uint32_t vlo = (skv + stage * kTile) >> 4, v_stage = stage;
+                    const bool more = j + 1 < mine;
+                    ok = j >= n0 - 1 ? wait_all(&v_clean[(clean + j - (n0 - 1)) % kPkClean], (clean + j - (n0 - 1)) / kPkClean) : full();
                     advance();
-                };
-                bool ok = true;
-                Item it;
-                for (uint32_t k = 0; ok && next_item(k, it, true); ++k) {
-                    const uint32_t n0 = tiles0(it), n1 = tiles1(it), n = max(n0, n1), mine = w ? n1 : n0;
-                    if (mine) {
-                        ok = wait(&q_full[w], done) && full();
-                        // Row tile 1 sets out when tile 0's first weights are done: in step, the two would
-                        // want the same pipes at the same time and leave them idle together.
-                        if (ok && w) ok = wait(&lead, done);
-                        if (!ok) break;
-                        fence_after();
-                        qk(mine == 1);
-                    }
-                    for (uint32_t j = 0; j < mine; ++j, ++steps) {
-                        // V tile j, then K tile j + 1 of the ring; what is there early is waited for early
-                        const uint32_t vlo = (skv + stage * kTile) >> 4, v_stage = stage;
-                        const bool more = j + 1 < mine;
-                        ok = j >= n0 - 1 ? wait(&v_clean[(clean + j - (n0 - 1)) % kPkClean], (clean + j - (n0 - 1)) / kPkClean) : full();
-                        advance();
-                        ok = ok && (!more || full());
-                        if (ok && j == 0 && done) ok = wait(&o_empty[w], done - 1);
-                        ok = ok && wait(&p_full[w][0], steps);
-                        if (!ok) break;
-                        fence_after();
+                    ok = ok && (!more || full());
+                    if (ok && j == 0 && done) ok = wait_all(&o_empty[w], done - 1);
+                    ok = ok && wait_all(&p_full[w][0], steps);
+                    if (!ok) break;
+                    fence_after();
+                    if (lead_lane) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i)
-                            mma_ts(to, tp + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), j | i);
-                        ok = wait(&p_full[w][1], steps);
-                        if (!ok) break;
-                        fence_after();
+                        for (uint32_t i = 0; i < 4; ++i) mma_ts(to, tp + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), j | i);
+                    }
+                    ok = wait_all(&p_full[w][1], steps);
+                    if (!ok) break;
+                    fence_after();
+                    if (lead_lane) {
 #pragma unroll
                         for (uint32_t i = 4; i < 8; ++i) mma_ts(to, tp + 8 * i, desc_mn(vlo + i * 128), idesc<BF16>(D, true), 1);
-                        if (more)
-                            qk(j + 2 == mine);
-                        else
-                            commit(&o_full[w]);
-                        commit(&kv_empty[v_stage]);
                     }
-                    if (!ok) break;
-                    done += mine != 0;
-                    // tiles that only the other row tile uses: released once they are there, in the ring's order
-                    for (uint32_t j = 2 * mine; j < 2 * n && ok; ++j) {
-                        ok = full();
-                        if (ok) mbar_arrive(&kv_empty[stage]);
-                        advance();
-                    }
-                    clean += n - (n0 - 1);
+                    if (more)
+                        qk(j + 2 == mine);
+                    else if (lead_lane)
+                        commit(&o_full[w]);
+                    if (lead_lane) commit(&kv_empty[v_stage]);
                 }
-                // every product complete before TMEM and the tiles are released
+                if (!ok) break;
+                done += mine != 0;
+                // tiles that only the other row tile uses: released once they are there, in the ring's order
+                for (uint32_t j = 2 * mine; j < 2 * n && ok; ++j) {
+                    ok = full();
+                    if (ok && lead_lane) mbar_arrive(&kv_empty[stage]);
+                    advance();
+                }
+                clean += n - (n0 - 1);
+            }
+            // every product complete before TMEM and the tiles are released
+            if (lead_lane) {
                 commit(&drain[w]);
                 mbar_drain(&drain[w], 0);
             }

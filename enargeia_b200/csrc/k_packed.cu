@@ -17,7 +17,7 @@
 // are f32.  Weights are rounded to the inputs' 16 bits for the product, as the output is.
 //
 // Bound: one exponential per score against 4 hd multiply-adds.  At 16 a clock and SM, 128 x 128 scores
-// are 1024 clocks, their products 512 at hd 64 and 1024 at hd 128; so three of eight exponentials are
+// are 1024 clocks, their products 512 at hd 64 and 1024 at hd 128; so at hd 128 some exponentials are
 // taken on the FMA pipe instead (2^x = 2^n 2^f, a cubic in f).
 //
 // One CTA per SM works through items, the next one's loads and first products under the present one's
@@ -59,7 +59,7 @@ constexpr uint32_t kPkThreads = 512;
 constexpr uint32_t kPkItems = 4;             // items between the warp that finds them and the others
 constexpr uint32_t kPkClean = 4;             // barriers of partly seen V tiles: more than a ring holds
 constexpr uint32_t kPkTileBytes = 128 * 128;  // 128 rows of 64 16-bit elements
-constexpr int kPkRegs = 128, kPkRegsSoftmax = 192, kPkRegsOut = 80, kPkRegsRest = 48;
+constexpr int kPkRegs = 128, kPkRegsSoftmax = 200, kPkRegsOut = 72, kPkRegsRest = 40;
 static_assert(2 * kPkRegsSoftmax + kPkRegsOut + kPkRegsRest <= 4 * kPkRegs, "the warpgroups' registers come out of the launch's");
 
 template <int D>
@@ -71,6 +71,10 @@ struct PackedShape {
     // TMEM columns of row tile w: S, P and O.  At hd 64 P has columns of its own, and the next scores are
     // multiplied while the present ones become weights; at hd 128 there is room only over S.
     static constexpr bool kApart = D == 64;
+    // One of so many pairs of exponentials is taken on the FMA pipe (0: none).  16384 keys, 16/2 heads, two
+    // row tiles in step: hd 64 717 TFLOP/s without, 702 with one of 8, 685 with one of 4; hd 128, whose
+    // products wait for the softmax, 1024 without, 1213 with one of 8, 1188 with one of 4.
+    static constexpr int kPolyOf = D == 64 ? 0 : 8;
     static constexpr uint32_t s_col(uint32_t w) { return kApart ? w * 256 : w * 128; }
     static constexpr uint32_t p_col(uint32_t w) { return kApart ? w * 256 + 128 : w * 128; }
     static constexpr uint32_t o_col(uint32_t w) { return kApart ? w * 256 + 192 : 256 + w * 128; }
@@ -188,6 +192,20 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
         "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
         "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t (&r)[16], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -364,40 +382,34 @@ __global__ void __launch_bounds__(kPkThreads, 1)
         for (uint32_t k = 0; ok && next_item(k, it, false); ++k) {
             const uint32_t tiles = w ? tiles1(it) : tiles0(it);
             if (!tiles) continue;
-            float m = 0.f;
+            float m = 0.f, mc = 0.f;  // the reference, and what it takes off a score in the exponent
             Pair l2 = pair(0.f, 0.f), l3 = l2;
-            for (uint32_t j = 0; j < tiles; ++j, ++steps) {
-                ok = __all_sync(0xffffffffu, wait(&s_full[w], steps));
-                if (!ok) break;
-                fence_after();
-                uint32_t s[4][32];
+            // 64 scores from column `at` on, key columns beyond the row's own unseen where that is the diagonal
+            auto mask = [&](uint32_t (&s)[2][32], uint32_t at) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld32(s[i], ts + 32 * i);
-                tmem_wait_ld();
-                if (Sh::kApart) {
-                    fence_before();
-                    mbar_arrive(&s_free[w]);
-                }
-                if (j + 1 == tiles) {  // the diagonal: key column > row is not seen
-#pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if ((uint32_t)i > row) s[i / 32][i % 32] = 0xff800000u;
-                }
+                for (int i = 0; i < 64; ++i)
+                    if (at + i > row) s[i / 32][i % 32] = 0xff800000u;
+            };
+            auto largest = [&](const uint32_t (&s)[2][32]) {
                 float top[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    top[i] = __uint_as_float(s[i][0]);
+                    const uint32_t* q = &s[i / 2][i % 2 * 16];
+                    top[i] = __uint_as_float(q[0]);
 #pragma unroll
-                    for (int e = 1; e < 31; e += 2) top[i] = max3(top[i], __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+                    for (int e = 1; e < 15; e += 2) top[i] = max3(top[i], __uint_as_float(q[e]), __uint_as_float(q[e + 1]));
+                    top[i] = max3(top[i], __uint_as_float(q[15]), top[i]);
                 }
-                float mx = max3(top[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
-                mx = max3(mx, __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
-                mx = max3(max3(mx, top[1], top[2]), top[3], mx);
-                // NaN among the scores stays NaN in the maximum, and infinity makes one, as inf - inf: the
-                // whole row is NaN then, whichever way its exponentials are taken
+                return max3(max3(top[0], top[1], top[2]), top[3], top[0]);
+            };
+            // The reference after key tile `tile`'s largest score mx.  NaN among the scores stays NaN in the maximum,
+            // and infinity makes one, as inf - inf: the whole row is NaN then, whichever way its exponentials are
+            // taken.  Where the reference moves, the row's sums so far are scaled, those in TMEM once the product
+            // of `before` steps is complete (hd 128: it is, as the scores were issued behind it).
+            auto settle = [&](float mx, uint32_t tile, uint32_t before) {
                 if (mx == INFINITY) mx = __int_as_float(0x7fffffff);
-                const bool move = j == 0 || !((mx - m) * c <= 8.f);
-                if (j == 0) {
+                const bool move = tile == 0 || !((mx - m) * c <= 8.f);
+                if (tile == 0) {
                     m = mx;
                 } else if (__any_sync(0xffffffffu, move)) {  // each row by itself: none depends on its neighbours
                     const float m_new = move ? max3(m, mx, mx) : m, f = move && m_new != -INFINITY ? ex2((m - m_new) * c) : 1.f;
@@ -407,63 +419,83 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                     l2 = pair(x * f, y * f);
                     unpair(l3, x, y);
                     l3 = pair(x * f, y * f);
-                    // (hd 128: the last key tile's product is complete, as these scores were issued after it)
                     if (Sh::kApart) {
-                        ok = __all_sync(0xffffffffu, wait(&pv_done[w], steps - 1));
-                        if (!ok) break;
+                        if (!__all_sync(0xffffffffu, wait(&pv_done[w], before))) return false;
                         fence_after();
                     }
 #pragma unroll 1
-                    for (uint32_t d = 0; d < D; d += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(o, to + d);
+                    for (uint32_t d = 0; d < D; d += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o, to + d);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st32(to + d, o);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(to + d, o);
                     }
                 }
-                const float mc = m == -INFINITY ? 0.f : -m * c;
+                mc = m == -INFINITY ? 0.f : -m * c;
+                return true;
+            };
+            // n weights in pairs, from pair i0 of 64 scores on, into p
+            auto weights = [&](const uint32_t (&s)[2][32], int i0, uint32_t* p, int n) {
                 const Pair cc = pair(c, c), mm = pair(mc, mc);
-                // weights i0 .. i0 + n of the row's 64 pairs, into p
-                auto weights = [&](uint32_t* p, int i0, int n) {
 #pragma unroll
-                    for (int i = 0; i < n; ++i) {
-                        const uint32_t e = 2 * (i0 + i);
-                        const Pair t = fma2(pair(__uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1])), cc, mm);
-                        float x, y;
-                        if (i % 8 == 1 || i % 8 == 4 || i % 8 == 6) {
-                            ex2_poly(t, x, y);
-                        } else {
-                            unpair(t, x, y);
-                            x = ex2(x);
-                            y = ex2(y);
-                        }
-                        if (i & 1)
-                            l3 = add2(l3, pair(x, y));
-                        else
-                            l2 = add2(l2, pair(x, y));
-                        p[i] = pack2<BF16>(x, y);
+                for (int i = 0; i < n; ++i) {
+                    const uint32_t e = 2 * (i0 + i);
+                    const Pair t = fma2(pair(__uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1])), cc, mm);
+                    float x, y;
+                    if (Sh::kPolyOf && i % (Sh::kPolyOf ? Sh::kPolyOf : 1) == 1) {
+                        ex2_poly(t, x, y);
+                    } else {
+                        unpair(t, x, y);
+                        x = ex2(x);
+                        y = ex2(y);
                     }
-                };
-                uint32_t p[2][32];
-                weights(p[0], 0, 32);
+                    if (i & 1)
+                        l3 = add2(l3, pair(x, y));
+                    else
+                        l2 = add2(l2, pair(x, y));
+                    p[i] = pack2<BF16>(x, y);
+                }
+            };
+            auto load = [&](uint32_t (&s)[2][32], uint32_t at) {
+                tmem_ld32(s[0], ts + at);
+                tmem_ld32(s[1], ts + at + 32);
+            };
+            uint32_t a0[2][32], a1[2][32], p[32];  // the two halves of a row's scores, and 64 weights
+            for (uint32_t j = 0; j < tiles; ++j, ++steps) {
+                ok = __all_sync(0xffffffffu, wait(&s_full[w], steps));
+                if (!ok) break;
+                fence_after();
+                load(a0, 0);
+                load(a1, 64);
+                tmem_wait_ld();
+                if (Sh::kApart) {
+                    fence_before();
+                    mbar_arrive(&s_free[w]);
+                }
+                if (j + 1 == tiles) {
+                    mask(a0, 0);
+                    mask(a1, 64);
+                }
+                const float mx = largest(a0);
+                ok = settle(max3(mx, largest(a1), mx), j, steps - 1);
+                if (!ok) break;
+                weights(a0, 0, p, 32);
                 if (Sh::kApart && steps) {  // the last weights have been used
                     ok = __all_sync(0xffffffffu, wait(&pv_done[w], steps - 1));
                     if (!ok) break;
                     fence_after();
                 }
-                tmem_st32(tp, p[0]);
-                if (Sh::kApart) {
-                    weights(p[1], 32, 32);
-                } else {  // the products of the first 64 keys begin under the last weights
-                    weights(p[1], 32, 16);
+                tmem_st32(tp, p);
+                weights(a1, 0, p, 16);
+                if (!Sh::kApart) {  // the products of the first 64 keys begin under the last weights
                     tmem_wait_st();
                     fence_before();
                     mbar_arrive(&p_full[w][0]);
-                    weights(p[1] + 16, 48, 16);
                 }
-                tmem_st32(tp + 32, p[1]);
+                weights(a1, 16, p + 16, 16);
+                tmem_st32(tp + 32, p);
                 tmem_wait_st();
                 fence_before();
                 mbar_arrive(&p_full[w][1]);

@@ -40,13 +40,36 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// The smallest and the largest of three, NaN if one is.
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// The whole number from 0 to 15 nearest to (x - m) / s, ties to even, where c is within one of it.  Exact: x -
+// m is split into its f32 value and the rest (two-sum), and the sign of x - m - (k + 1/2) s, with k + 1/2 the
+// border on that side of c on which the value lies, decides; the FMA's result has the sign of the exact one.
+__device__ __forceinline__ float nearest_code(float x, float m, float s, float c) {
+    const float d = x - m, back = d - x, rest = (x - (d - back)) - (m + back);
+    const float side = fmaf(-c, s, d) + rest < 0.f ? -0.5f : 0.5f, at = c + side;
+    const float over = fmaf(-at, s, d) + rest;  // how far the value lies above that border
+    const bool odd = (int)c & 1, beyond = side > 0.f ? over > 0.f : over < 0.f;
+    return fminf(fmaxf(beyond || (over == 0.f && odd) ? c + 2.f * side : c, 0.f), 15.f);
+}
+
 struct WriteArgs {
     const void *k, *v;
     void *k_out, *v_out;  // contiguous [tokens][kv_heads][hd], or null
     long long k_token, k_head, v_token, v_head;  // strides in elements
     uint8_t* pool;
     const int32_t *table, *seqs, *positions;
-    uint32_t tokens, rows, width, pages, page_shift, kv_heads, hd;
+    uint32_t tokens, rows, width, pages, page_shift, kv_heads, hd, head_shift;
     int vec;  // all rows start on 16 bytes
 };
 
@@ -54,99 +77,116 @@ struct WriteArgs {
 
 // Eight elements per thread, 4 (hd 32) or 8 threads per group.  HBM-bound: rows in, codes and the
 // values they stand for out.  The f16 scale and the codes are decided exactly: quotients are taken
-// in f32, and again in f64 where f32 cannot tell on which side of a border they lie.  A group with
+// in f32, and settled without rounding where f32 cannot tell on which side of a border they lie.  A group with
 // an element that is not finite gets NaN parameters, so that what reads it is not finite either.
+//
+// What it costs otherwise is instructions: K and V of a place share the search for it, rounding and packing
+// are additions and FMAs, not conversions and shifts, and the rows are fetched while their place is still
+// looked up.
 template <typename T>
 __global__ void __launch_bounds__(256) k_kv4_write(WriteArgs a) {
-    const uint32_t per_head = a.hd / 8, per_token = 2 * a.kv_heads * per_head;
+    // thread = 8 elements of one token and head, of K and of V
     const uint32_t item = blockIdx.x * 256 + threadIdx.x;  // below 2^32: the host refuses more
-    const uint32_t token = item / per_token, u = item % per_token, kv = u / (per_token / 2), hu = u % (per_token / 2);
-    const uint32_t head = hu / per_head, e8 = hu % per_head;
+    const uint32_t row = item >> a.head_shift, e8 = item & (a.hd / 8 - 1);
+    const uint32_t token = row / a.kv_heads, head = row - token * a.kv_heads;
     bool live = token < a.tokens;
-    const int32_t pos = live ? a.positions[token] : -1, seq = live ? a.seqs[token] : -1;
-    int32_t page = -1;
-    if (pos >= 0 && seq >= 0 && (uint32_t)seq < a.rows && ((uint32_t)pos >> a.page_shift) < a.width)
-        page = a.table[(size_t)seq * a.width + ((uint32_t)pos >> a.page_shift)];
-    live = page >= 0 && (uint32_t)page < a.pages;
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    alignas(16) T raw[2][8];
+    int32_t pos = -1, seq = -1, page = -1;
     if (live) {
-        const T* src = static_cast<const T*>(kv ? a.v : a.k) + (long long)token * (kv ? a.v_token : a.k_token) +
-                       (long long)head * (kv ? a.v_head : a.k_head) + e8 * 8;
-        if (a.vec) {
-            alignas(16) T tmp[8];
+        pos = a.positions[token];
+        seq = a.seqs[token];
 #pragma unroll
-            for (uint32_t i = 0; i < sizeof(T) / 2; ++i)
-                reinterpret_cast<uint4*>(tmp)[i] = ld_stream(reinterpret_cast<const uint4*>(src) + i);
+        for (int kv = 0; kv < 2; ++kv) {
+            const T* src = static_cast<const T*>(kv ? a.v : a.k) + (long long)token * (kv ? a.v_token : a.k_token) +
+                           (long long)head * (kv ? a.v_head : a.k_head) + e8 * 8;
+            if (a.vec) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = to_f(tmp[i]);
-        } else {
+                for (uint32_t i = 0; i < sizeof(T) / 2; ++i)
+                    reinterpret_cast<uint4*>(raw[kv])[i] = ld_stream(reinterpret_cast<const uint4*>(src) + i);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = to_f(src[i]);
+                for (int i = 0; i < 8; ++i) raw[kv][i] = src[i];
+            }
         }
-    }
-    float lo = x[0], hi = x[0];
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        finite = finite && isfinite(x[i]);
-    }
-    const uint32_t lanes = a.hd < 64 ? 4 : 8;  // of a group (whole groups lie in a warp)
-    for (uint32_t o = 1; o < lanes; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        finite = __shfl_xor_sync(0xffffffffu, (int)finite, o) && finite;
-    }
-    if (!live) return;
-    __half sc, of;
-    if (finite) {
-        // the f32 quotient is off by less than 2^-21 of itself (difference, product, 1/15)
-        const float q = (hi - lo) * (1.f / 15.f);
-        sc = __float2half_rn(fminf(q * (1.f - 0x1p-20f), 65504.f));
-        if (__half_as_ushort(sc) != __half_as_ushort(__float2half_rn(fminf(q * (1.f + 0x1p-20f), 65504.f))))
-            sc = __float2half_rn((float)fmin(((double)hi - (double)lo) / 15.0, 65504.0));
-        of = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
+        if (pos >= 0 && seq >= 0 && (uint32_t)seq < a.rows && ((uint32_t)pos >> a.page_shift) < a.width)
+            page = a.table[(size_t)seq * a.width + ((uint32_t)pos >> a.page_shift)];
     } else {
-        sc = of = __ushort_as_half(0x7e00);  // NaN
-    }
-    const float s = __half2float(sc), m = __half2float(of);
-    uint32_t word = 0;
-    float val[8];
-    const float inv = 1.f / s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float c = 0.f;
-        if (s > 0.f) {
-            const float t = (x[i] - m) * inv;
-            c = rintf(t);
-            // t < 17 is off by less than 17 * 3 * 2^-24 < 2^-18 (difference, inverse, product)
-            if (fabsf(fabsf(t - c) - 0.5f) < 0x1p-17f && t < 17.f) c = (float)rint(((double)x[i] - (double)m) / (double)s);
-            c = fminf(fmaxf(c, 0.f), 15.f);
-        }
-        word |= (uint32_t)c << (4 * i);
-        val[i] = fmaf(s, c, m);
+        for (int i = 0; i < 16; ++i) raw[i / 8][i % 8] = from_f<T>(0.f);
     }
+    live = page >= 0 && (uint32_t)page < a.pages;
+    const uint32_t lanes = a.hd < 64 ? 4 : 8;  // of a group (whole groups lie in a warp)
     const uint32_t groups = a.hd > 64 ? a.hd / 64 : 1, pt = 1u << a.page_shift, slot = (uint32_t)pos & (pt - 1);
     const uint32_t head_bytes = pt * (a.hd + 8 * groups);
-    uint8_t* at = a.pool + ((size_t)(uint32_t)page * a.kv_heads + head) * head_bytes + (kv ? head_bytes / 2 : 0);
-    *reinterpret_cast<uint32_t*>(at + slot * (a.hd / 2) + e8 * 4) = word;
-    if (e8 % lanes == 0)
-        *reinterpret_cast<__half2*>(at + pt * (a.hd / 2) + (slot * groups + e8 / lanes) * 4) = __halves2half2(sc, of);
-    void* back = kv ? a.v_out : a.k_out;
-    if (back) {
-        T* dst = static_cast<T*>(back) + ((size_t)token * a.kv_heads + head) * a.hd + e8 * 8;
-        alignas(16) T tmp[8];
+    uint8_t* at = a.pool + ((size_t)(uint32_t)max(page, 0) * a.kv_heads + head) * head_bytes;
+    const size_t back_at = ((size_t)token * a.kv_heads + head) * a.hd + e8 * 8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) tmp[i] = from_f<T>(val[i]);
-        if (a.vec) {
+    for (int kv = 0; kv < 2; ++kv) {
+        float x[8];
 #pragma unroll
-            for (uint32_t i = 0; i < sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(tmp)[i];
+        for (int i = 0; i < 8; ++i) x[i] = to_f(raw[kv][i]);
+        float lo = min3(min3(min3(x[0], x[1], x[2]), x[3], x[4]), min3(x[5], x[6], x[7]), x[0]);
+        float hi = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), x[0]);
+#pragma unroll
+        for (uint32_t o = 1; o < 8; o <<= 1)
+            if (o < lanes) {
+                const float l = __shfl_xor_sync(0xffffffffu, lo, o), h = __shfl_xor_sync(0xffffffffu, hi, o);
+                lo = min3(lo, l, l);
+                hi = max3(hi, h, h);
+            }
+        if (!live) continue;
+        __half sc, of;
+        if (fabsf(lo) < INFINITY && fabsf(hi) < INFINITY) {  // (both are NaN where an element is)
+            // the f32 quotient is off by less than 2^-21 of itself (difference, product, 1/15)
+            const float q = (hi - lo) * (1.f / 15.f);
+            sc = __float2half_rn(fminf(q * (1.f - 0x1p-20f), 65504.f));
+            if (__half_as_ushort(sc) != __half_as_ushort(__float2half_rn(fminf(q * (1.f + 0x1p-20f), 65504.f))))
+                sc = __float2half_rn((float)fmin(((double)hi - (double)lo) / 15.0, 65504.0));
+            of = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
         } else {
+            sc = of = __ushort_as_half(0x7e00);  // NaN
+        }
+        const float s = __half2float(sc), m = __half2float(of);
+        const float inv15 = s > 0.f ? __fdividef(1.f / 15.f, s) : 0.f;  // 0: every code is 0
+        constexpr float kWhole = 12582912.f;                             // 1.5 * 2^23: added, it rounds to whole numbers
+        float c[8], val[8];
+        bool border = false;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[i] = tmp[i];
+        for (int i = 0; i < 8; ++i) {
+            const float u = __saturatef((x[i] - m) * inv15);  // the code before rounding, in fifteenths
+            c[i] = fmaf(u, 15.f, kWhole) - kWhole;
+            // 15 u is off by less than 15 * 6 * 2^-24 < 2^-17 (difference, quotient of 2 ulp, 1/15, product, FMA);
+            // borders are at c +- 1/2
+            border = border || fabsf(fmaf(u, 15.f, -c[i])) > 0.5f - 0x1p-16f;
+        }
+        if (border) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (s > 0.f) c[i] = nearest_code(x[i], m, s, c[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) val[i] = fmaf(s, c[i], m);
+        // four codes at a time are a whole number below 2^16, exactly
+        const float w0 = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f;
+        const float w1 = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 8388608.f;
+        const uint32_t word = __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x5410);
+        uint8_t* half = at + (kv ? head_bytes / 2 : 0);
+        *reinterpret_cast<uint32_t*>(half + slot * (a.hd / 2) + e8 * 4) = word;
+        if ((e8 & (lanes - 1)) == 0)
+            *reinterpret_cast<__half2*>(half + pt * (a.hd / 2) + (slot * groups + (lanes == 8 ? e8 >> 3 : 0)) * 4) = __halves2half2(sc, of);
+        T* back = static_cast<T*>(kv ? a.v_out : a.k_out);
+        if (back) {
+            alignas(16) T tmp[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) tmp[i] = from_f<T>(val[i]);
+            if (a.vec) {
+#pragma unroll
+                for (uint32_t i = 0; i < sizeof(T) / 2; ++i)
+                    reinterpret_cast<uint4*>(back + back_at)[i] = reinterpret_cast<const uint4*>(tmp)[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) back[back_at + i] = tmp[i];
+            }
         }
     }
 }
@@ -1012,20 +1052,21 @@ extern "C" enx_status enx_kv4_write(const void* k, const void* v, const int64_t*
         return fail(ENX_ERR_INVALID, "enx_kv4_write: null pointer");
     if (reinterpret_cast<uintptr_t>(pool) % 16) return fail(ENX_ERR_INVALID, "enx_kv4_write: the pool must be 16-byte aligned");
     WriteArgs a{k, v, k_out, v_out, strides[0], strides[1], strides[2], strides[3], pool, table, seqs, positions, tokens,
-                d->rows, d->width, d->pages, log2_of(d->page_tokens), d->kv_heads, d->head_dim, 0};
+                d->rows, d->width, d->pages, log2_of(d->page_tokens), d->kv_heads, d->head_dim, log2_of(d->head_dim / 8), 0};
     const size_t size = d->dtype == ENX_F32 ? 4 : 2;
     uintptr_t any = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_out) |
                     reinterpret_cast<uintptr_t>(v_out);
     for (int i = 0; i < 4; ++i) any |= (uintptr_t)strides[i] * size;
     a.vec = any % 16 == 0;
-    const uint64_t threads = (uint64_t)tokens * 2 * d->kv_heads * (d->head_dim / 8), blocks = (threads + 255) / 256;
+    const uint64_t threads = (uint64_t)tokens * d->kv_heads * (d->head_dim / 8), blocks = (threads + 255) / 256;
+    const uint32_t grid = (uint32_t)blocks;
     if (blocks * 256 > 0xffffffffull) return fail(ENX_ERR_RANGE, "enx_kv4_write: too many tokens for one call");
     if (d->dtype == ENX_F32)
-        k_kv4_write<float><<<(uint32_t)blocks, 256, 0, as_stream(stream)>>>(a);
+        k_kv4_write<float><<<grid, 256, 0, as_stream(stream)>>>(a);
     else if (d->dtype == ENX_F16)
-        k_kv4_write<__half><<<(uint32_t)blocks, 256, 0, as_stream(stream)>>>(a);
+        k_kv4_write<__half><<<grid, 256, 0, as_stream(stream)>>>(a);
     else
-        k_kv4_write<__nv_bfloat16><<<(uint32_t)blocks, 256, 0, as_stream(stream)>>>(a);
+        k_kv4_write<__nv_bfloat16><<<grid, 256, 0, as_stream(stream)>>>(a);
     ENX_CUDA(cudaGetLastError());
     return ENX_OK;
 }

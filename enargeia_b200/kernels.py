@@ -7,6 +7,7 @@ C ABI directly.  torch is only the allocator and stream provider here.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -142,18 +143,26 @@ def add(a, b, out, stream=None):
 
 
 # ---- pages of a shared key/value cache -----------------------------------------------------------
+#
+# These calls take a few microseconds on the GPU, so their checks are kept short: one look at each
+# tensor, and argument blocks that only depend on sizes are made once per sizes.
+
+_INT32 = torch.int32
 
 
-def _i32(t: torch.Tensor, *shape) -> int:
-    """Address of a contiguous int32 CUDA tensor, of this shape (None: any size there)."""
-    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
-        raise ValueError("expected a contiguous int32 CUDA tensor")
-    if t.shape != shape and (len(shape) != t.dim() or any(w is not None and w != g for w, g in zip(shape, t.shape))):
-        raise ValueError(f"expected an int32 tensor of shape {shape}, got {tuple(t.shape)}")
+def _ints(t: torch.Tensor, n: int) -> int:
+    """Address of a contiguous int32 CUDA tensor of n entries."""
+    if t.dtype is not _INT32 or t.numel() != n or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"expected a contiguous int32 CUDA tensor of {n} entries, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _call_on(tensors, name: str, *args, stream=None) -> None:
+#: The current device and the current stream's handle, without the objects around them.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call_on(tensors, stream, name: str, *args) -> None:
     """`call` with the stream appended, on the device that all the tensors (None: absent) are on."""
     index = tensors[0].get_device()
     for t in tensors:
@@ -161,15 +170,10 @@ def _call_on(tensors, name: str, *args, stream=None) -> None:
             raise ValueError(f"expected all tensors on one device, got {tensors[0].device} and {t.device}")
     if index < 0:
         raise ValueError("expected CUDA tensors")
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
-            return call(name, *args, _stream(stream))
+            return call(name, *args, _raw_stream(index) if stream is None else stream.cuda_stream)
     call(name, *args, _raw_stream(index) if stream is None else stream.cuda_stream)
-
-
-#: The current stream's handle without the Stream object around it (a few us less a call).
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _enough(workspace: Optional[torch.Tensor], nbytes: int, like: torch.Tensor, stream) -> torch.Tensor:
@@ -178,15 +182,15 @@ def _enough(workspace: Optional[torch.Tensor], nbytes: int, like: torch.Tensor, 
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
         if stream is not None:
             workspace.record_stream(stream)
-    elif workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous():
-        raise ValueError(f"the workspace has to have {nbytes} contiguous bytes")
+    elif workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous() or not workspace.is_cuda:
+        raise ValueError(f"the workspace has to have {nbytes} contiguous bytes on the device")
     return workspace
 
 
-def _pages_dims(table, lengths, refs, status, page_tokens):
-    rows, width = table.shape
-    return (_i32(table, None, None), _i32(lengths, rows), _i32(refs, None), _i32(status, 1),
-            PagesDims(rows, width, refs.numel(), page_tokens))
+@lru_cache(maxsize=256)
+def _pages_block(rows, width, pages, page_tokens):
+    """(argument block, workspace bytes) of the page calls."""
+    return C.byref(PagesDims(rows, width, pages, page_tokens)), _lib.load().enx_pages_workspace_bytes(rows, pages)
 
 
 def pages_free(table, lengths, refs, rows, keep, status, page_tokens, stream=None):
@@ -194,53 +198,58 @@ def pages_free(table, lengths, refs, rows, keep, status, page_tokens, stream=Non
 
     table int32 [rows, width], lengths int32 [rows], refs int32 [pages] (holders of each page) and
     status int32 [1] (error bits of include/enx.h, added to) are the cache's state; lists are int32."""
-    t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
-    n = rows.numel()
-    _call_on((table, lengths, refs, rows, keep, status), "enx_pages_free", t, l, r, _i32(rows, n), _i32(keep, n), n, st,
-             C.byref(d), stream=stream)
+    r, w = table.shape
+    n, p = rows.numel(), refs.numel()
+    _call_on((table, lengths, refs, rows, keep, status), stream, "enx_pages_free", _ints(table, r * w), _ints(lengths, r),
+             _ints(refs, p), _ints(rows, n), _ints(keep, n), n, _ints(status, 1), _pages_block(r, w, p, page_tokens)[0])
 
 
 def pages_fork(table, lengths, refs, src, dst, status, page_tokens, stream=None):
     """Empty rows `dst` become further holders of the pages of rows `src`."""
-    t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
-    n = dst.numel()
-    _call_on((table, lengths, refs, src, dst, status), "enx_pages_fork", t, l, r, _i32(src, n), _i32(dst, n), n, st,
-             C.byref(d), stream=stream)
+    r, w = table.shape
+    n, p = dst.numel(), refs.numel()
+    _call_on((table, lengths, refs, src, dst, status), stream, "enx_pages_fork", _ints(table, r * w), _ints(lengths, r),
+             _ints(refs, p), _ints(src, n), _ints(dst, n), n, _ints(status, 1), _pages_block(r, w, p, page_tokens)[0])
 
 
 def pages_grow(table, lengths, refs, rows, add, pairs, count, status, page_tokens, workspace=None, stream=None):
     """Room for `add` more tokens in rows `rows`; pairs int32 [n, 2] and count int32 [2] say which
     pages to copy before they are written (`pages_copy`) and how many pages were taken."""
-    t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
-    n = rows.numel()
-    if pairs.shape[0] < n:
+    r, w = table.shape
+    n, p = rows.numel(), refs.numel()
+    if pairs.numel() < 2 * n:
         raise ValueError(f"pairs has to have {n} rows")
-    ws = _enough(workspace, _lib.load().enx_pages_workspace_bytes(d.rows, d.pages), table, stream)
-    _call_on((table, lengths, refs, rows, add, pairs, count, status, ws), "enx_pages_grow", t, l, r, _i32(rows, n),
-             _i32(add, n), n, _i32(pairs, None, 2), _i32(count, 2), st, C.byref(d), _ptr(ws), stream=stream)
+    block, nbytes = _pages_block(r, w, p, page_tokens)
+    ws = _enough(workspace, nbytes, table, stream)
+    _call_on((table, lengths, refs, rows, add, pairs, count, status, ws), stream, "enx_pages_grow", _ints(table, r * w),
+             _ints(lengths, r), _ints(refs, p), _ints(rows, n), _ints(add, n), n, _ints(pairs, pairs.shape[0] * 2), _ints(count, 2),
+             _ints(status, 1), block, ws.data_ptr())
 
 
 def pages_compact(table, lengths, refs, table_out, refs_out, pairs, count, status, page_tokens, workspace=None,
                   stream=None):
     """Closes the used pages up to the front: the table and the counts under the new numbers, pairs
     int32 [pages, 2] of pages to copy, count = (pairs, pages in use)."""
-    t, l, r, st, d = _pages_dims(table, lengths, refs, status, page_tokens)
-    if pairs.shape[0] < d.pages:
-        raise ValueError(f"pairs has to have {d.pages} rows")
-    ws = _enough(workspace, _lib.load().enx_pages_workspace_bytes(d.rows, d.pages), table, stream)
-    _call_on((table, lengths, refs, table_out, refs_out, pairs, count, status, ws), "enx_pages_compact", t, l, r,
-             _i32(table_out, d.rows, d.width), _i32(refs_out, d.pages), _i32(pairs, None, 2), _i32(count, 2), st,
-             C.byref(d), _ptr(ws), stream=stream)
+    r, w = table.shape
+    p = refs.numel()
+    if pairs.numel() < 2 * p or table_out.shape != table.shape:
+        raise ValueError(f"pairs has to have {p} rows, and table_out the table's shape")
+    block, nbytes = _pages_block(r, w, p, page_tokens)
+    ws = _enough(workspace, nbytes, table, stream)
+    _call_on((table, lengths, refs, table_out, refs_out, pairs, count, status, ws), stream, "enx_pages_compact",
+             _ints(table, r * w), _ints(lengths, r), _ints(refs, p), _ints(table_out, r * w), _ints(refs_out, p),
+             _ints(pairs, pairs.shape[0] * 2), _ints(count, 2), _ints(status, 1), block, ws.data_ptr())
 
 
 def pages_copy(pool, pairs, count, status, stream=None):
     """Copies page pairs[i, 0] onto page pairs[i, 1] in every layer of pool uint8 [layers, pages,
     page bytes], for the first count[0] pairs."""
-    if pool.dtype != torch.uint8 or pool.dim() != 3:
-        raise ValueError("expected a uint8 pool [layers, pages, page bytes]")
     layers, pages, nbytes = pool.shape
-    _call_on((pool, pairs, count, status), "enx_pages_copy", _ptr(pool), layers, pages, nbytes, _i32(pairs, None, 2),
-             pairs.shape[0], _i32(count, None), _i32(status, 1), stream=stream)
+    if pool.dtype is not torch.uint8:
+        raise ValueError("expected a uint8 pool [layers, pages, page bytes]")
+    n = pairs.shape[0]
+    _call_on((pool, pairs, count, status), stream, "enx_pages_copy", _ptr(pool), layers, pages, nbytes, _ints(pairs, 2 * n), n,
+             _ints(count, count.numel()), _ints(status, 1))
 
 
 # ---- a paged cache held in 4 bits, and attention over it ---------------------------------------------
@@ -248,24 +257,33 @@ def pages_copy(pool, pairs, count, status, stream=None):
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _kv4_dims(pool, table, page_tokens, kv_heads, head_dim, dtype):
-    if dtype not in _DTYPES:
-        raise ValueError(f"expected float32, float16 or bfloat16, got {dtype}")
-    if pool.dtype != torch.uint8 or pool.dim() != 2:
-        raise ValueError("expected one layer's uint8 pool [pages, page bytes]")
-    if pool.shape[1] != kv4_page_bytes(page_tokens, kv_heads, head_dim):
-        raise ValueError(f"a page has {kv4_page_bytes(page_tokens, kv_heads, head_dim)} bytes, the pool's {pool.shape[1]}")
-    rows, width = table.shape
-    return Kv4Dims(rows, width, pool.shape[0], page_tokens, kv_heads, head_dim, _DTYPES[dtype], 0)
-
-
 def kv4_page_bytes(page_tokens: int, kv_heads: int, head_dim: int) -> int:
     """Bytes of a page of the 4-bit cache (one layer): codes and parameters of K and V."""
     return page_tokens * kv_heads * (head_dim + 8 * max(1, head_dim // 64))
 
 
+@lru_cache(maxsize=256)
+def _kv4_block(rows, width, pages, nbytes, page_tokens, kv_heads, head_dim, dtype):
+    """The argument block of the 4-bit cache's calls."""
+    if dtype not in _DTYPES:
+        raise ValueError(f"expected float32, float16 or bfloat16, got {dtype}")
+    if nbytes != kv4_page_bytes(page_tokens, kv_heads, head_dim):
+        raise ValueError(f"a page has {kv4_page_bytes(page_tokens, kv_heads, head_dim)} bytes, the pool's {nbytes}")
+    return C.byref(Kv4Dims(rows, width, pages, page_tokens, kv_heads, head_dim, _DTYPES[dtype], 0))
+
+
+@lru_cache(maxsize=256)
+def _strides(*elements):
+    return (C.c_int64 * len(elements))(*elements)
+
+
+@lru_cache(maxsize=64)
+def _attn_kv4_bytes(batch, head_dim):
+    return _lib.load().enx_attn_kv4_workspace_bytes(batch, head_dim)
+
+
 def _rows_of(t: torch.Tensor) -> int:
-    """Pointer of a CUDA tensor whose last axis is contiguous (its other strides go with the call)."""
+    """Address of a CUDA tensor whose last axis is contiguous (its other strides go with the call)."""
     if not t.is_cuda:
         raise ValueError("expected a CUDA tensor")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
@@ -273,40 +291,54 @@ def _rows_of(t: torch.Tensor) -> int:
     return t.data_ptr()
 
 
+def _pool_of(pool: torch.Tensor):
+    """(pages, page bytes) of one layer's pool."""
+    if pool.dtype is not torch.uint8 or pool.dim() != 2:
+        raise ValueError("expected one layer's uint8 pool [pages, page bytes]")
+    return pool.shape
+
+
 def kv4_write(k, v, pool, table, seqs, positions, page_tokens, k_out=None, v_out=None, stream=None):
     """Quantises k and v [tokens, kv_heads, head_dim] into the 4-bit cache: token i to position
     positions[i] of table row seqs[i] (int32; a negative position is passed over).  k_out and v_out,
     if given, receive the values that the cache now holds."""
-    tokens, kv_heads, hd = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype:
+    shape = k.shape
+    tokens, kv_heads, hd = shape
+    if v.shape != shape or v.dtype is not k.dtype:
         raise ValueError("k and v have to have one shape and type")
     for o in (k_out, v_out):
-        if o is not None and (o.shape != k.shape or o.dtype != k.dtype):
+        if o is not None and (o.shape != shape or o.dtype is not k.dtype):
             raise ValueError("k_out and v_out have to have the shape and type of k")
-    d = _kv4_dims(pool, table, page_tokens, kv_heads, hd, k.dtype)
-    strides = (C.c_int64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    _call_on((k, v, pool, table, seqs, positions, k_out, v_out), "enx_kv4_write", _rows_of(k), _rows_of(v), strides, tokens,
-             _ptr(pool), _i32(table, None, None), _i32(seqs, tokens), _i32(positions, tokens), _ptr(k_out), _ptr(v_out),
-             C.byref(d), stream=stream)
+    r, w = table.shape
+    pages, nbytes = _pool_of(pool)
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    _call_on((k, v, pool, table, seqs, positions, k_out, v_out), stream, "enx_kv4_write", _rows_of(k), _rows_of(v),
+             _strides(k0, k1, v0, v1), tokens, _ptr(pool), _ints(table, r * w), _ints(seqs, tokens), _ints(positions, tokens),
+             _ptr(k_out), _ptr(v_out), _kv4_block(r, w, pages, nbytes, page_tokens, kv_heads, hd, k.dtype))
 
 
 def attn_kv4(q, pool, table, lengths, out, kv_heads, page_tokens, seqs=None, scale=None, workspace=None, stream=None):
     """Attention of each sequence's newest tokens over its 4-bit cache: q and out [batch, queries,
     heads, head_dim] or [batch, heads, head_dim]; sequence b is table row seqs[b] (or b), and
     lengths[row] counts its tokens, the queries' own included."""
-    if q.shape != out.shape or q.dtype != out.dtype:
+    shape = q.shape
+    if shape != out.shape or q.dtype is not out.dtype:
         raise ValueError("q and out have to have one shape and type")
-    if q.dim() == 3:
-        q = q.unsqueeze(1)
-    batch, queries, heads, hd = q.shape
-    d = _kv4_dims(pool, table, page_tokens, kv_heads, hd, q.dtype)
-    if lengths.shape != (d.rows,):
-        raise ValueError("lengths has to have an entry for each table row")
-    ws = _enough(workspace, _lib.load().enx_attn_kv4_workspace_bytes(batch, hd), q, stream)
-    strides = (C.c_int64 * 3)(q.stride(0), q.stride(1), q.stride(2))
-    _call_on((q, pool, table, lengths, out, seqs, ws), "enx_attn_kv4", _rows_of(q), strides, _ptr(pool),
-             _i32(table, None, None), _i32(lengths, None), None if seqs is None else _i32(seqs, batch), _ptr(out), batch,
-             queries, heads, hd ** -0.5 if scale is None else scale, C.byref(d), _ptr(ws), stream=stream)
+    if len(shape) == 3:
+        batch, heads, hd = shape
+        queries, (s0, s2, _) = 1, q.stride()
+        s1 = 0
+    else:
+        batch, queries, heads, hd = shape
+        s0, s1, s2, _ = q.stride()
+    r, w = table.shape
+    pages, nbytes = _pool_of(pool)
+    ws = _enough(workspace, _attn_kv4_bytes(batch, hd), q, stream)
+    _call_on((q, pool, table, lengths, out, seqs, ws), stream, "enx_attn_kv4", _rows_of(q), _strides(s0, s1, s2), _ptr(pool),
+             _ints(table, r * w), _ints(lengths, r), None if seqs is None else _ints(seqs, batch), _ptr(out), batch, queries, heads,
+             hd ** -0.5 if scale is None else scale, _kv4_block(r, w, pages, nbytes, page_tokens, kv_heads, hd, q.dtype),
+             ws.data_ptr())
     return out
 
 
@@ -322,13 +354,13 @@ def attn_packed(q, k, v, out, offsets, scale=None, stream=None):
         raise ValueError("q and out have to have one shape, and k and v one with the same tokens and head_dim")
     if not (q.dtype is k.dtype is v.dtype is out.dtype):
         raise ValueError("q, k, v and out have to have one type")
-    strides = (C.c_int64 * 8)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                              out.stride(0), out.stride(1))
-    if offsets.numel() < 1:
+    n = offsets.numel()
+    if n < 1:
         raise ValueError("offsets has an entry more than there are prompts")
-    _call_on((q, k, v, out, offsets), "enx_attn_packed", _rows_of(q), _rows_of(k), _rows_of(v), _rows_of(out), strides,
-             _i32(offsets, None), offsets.numel() - 1, tokens, heads, kv_heads, hd, _DTYPES[q.dtype],
-             hd ** -0.5 if scale is None else scale, stream=stream)
+    (q0, q1, _), (k0, k1, _), (v0, v1, _), (o0, o1, _) = q.stride(), k.stride(), v.stride(), out.stride()
+    _call_on((q, k, v, out, offsets), stream, "enx_attn_packed", _rows_of(q), _rows_of(k), _rows_of(v), _rows_of(out),
+             _strides(q0, q1, k0, k1, v0, v1, o0, o1), _ints(offsets, n), n - 1, tokens, heads, kv_heads, hd, _DTYPES[q.dtype],
+             hd ** -0.5 if scale is None else scale)
     return out
 
 

@@ -59,7 +59,7 @@ constexpr uint32_t kPkThreads = 512;
 constexpr uint32_t kPkItems = 4;             // items between the warp that finds them and the others
 constexpr uint32_t kPkClean = 4;             // barriers of partly seen V tiles: more than a ring holds
 constexpr uint32_t kPkTileBytes = 128 * 128;  // 128 rows of 64 16-bit elements
-constexpr int kPkRegs = 128, kPkRegsSoftmax = 200, kPkRegsOut = 72, kPkRegsRest = 40;
+constexpr int kPkRegs = 128, kPkRegsSoftmax = 192, kPkRegsOut = 88, kPkRegsRest = 40;
 static_assert(2 * kPkRegsSoftmax + kPkRegsOut + kPkRegsRest <= 4 * kPkRegs, "the warpgroups' registers come out of the launch's");
 
 template <int D>
@@ -567,36 +567,41 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                 const bool live = at < it.len;
                 uint16_t* dst = static_cast<uint16_t*>(a.out) + (long long)(it.begin + at) * a.out_token + (long long)it.head * a.out_head;
 #pragma unroll 1
-                for (uint32_t d = 0; d < D; d += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(o, to + d);
+                for (uint32_t d = 0; d < D; d += 64) {
+                    // O is free for the next item as soon as it is in registers
+                    uint32_t o[2][32];
+                    tmem_ld32(o[0], to + d);
+                    tmem_ld32(o[1], to + d + 32);
                     tmem_wait_ld();
+                    if (d + 64 == D) {
+                        fence_before();
+                        mbar_arrive(&o_empty[w]);
+                    }
                     if (foul && live) {
                         // elements that are not finite, of the keys of the last two tiles that this row sees
                         const uint16_t* v = static_cast<const uint16_t*>(a.v) + (long long)(it.head / group) * a.v_head;
                         for (uint32_t key = it.pair * 256; key <= at; ++key) {
                             const uint16_t* vr = v + (long long)(it.begin + key) * a.v_token + d;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
+                            for (int i = 0; i < 64; ++i)
                                 if (d + i < a.hd && not_finite16<BF16>(vr[i]))
-                                    o[i] = __float_as_uint(__uint_as_float(o[i]) +
-                                                           (BF16 ? __uint_as_float((uint32_t)vr[i] << 16)
-                                                                 : __half2float(__ushort_as_half(vr[i]))));
+                                    o[i / 32][i % 32] = __float_as_uint(__uint_as_float(o[i / 32][i % 32]) +
+                                                                        (BF16 ? __uint_as_float((uint32_t)vr[i] << 16)
+                                                                              : __half2float(__ushort_as_half(vr[i]))));
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8)
+                    for (int i = 0; i < 64; i += 8)
                         if (live && d + i < a.hd) {
+                            const uint32_t* q = &o[i / 32][i % 32];
                             uint4 r;
-                            r.x = pack2<BF16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-                            r.y = pack2<BF16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                            r.z = pack2<BF16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-                            r.w = pack2<BF16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                            r.x = pack2<BF16>(__uint_as_float(q[0]) * inv, __uint_as_float(q[1]) * inv);
+                            r.y = pack2<BF16>(__uint_as_float(q[2]) * inv, __uint_as_float(q[3]) * inv);
+                            r.z = pack2<BF16>(__uint_as_float(q[4]) * inv, __uint_as_float(q[5]) * inv);
+                            r.w = pack2<BF16>(__uint_as_float(q[6]) * inv, __uint_as_float(q[7]) * inv);
                             *reinterpret_cast<uint4*>(dst + d + i) = r;
                         }
                 }
-                fence_before();
-                mbar_arrive(&o_empty[w]);
             }
         }
     } else {

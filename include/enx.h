@@ -333,14 +333,14 @@ ENX_API size_t enx_attn_kv4_workspace_bytes(uint32_t batch, uint32_t head_dim);
 
 /* Causal attention over whole prompts packed one behind another (the reference prefills one
  * sequence, in f32 over its f16 cache: src/kernels/cache_variants.ts:81-144): token i of prompt s
- * (rows offsets[s] to offsets[s + 1] - 1; offsets int32 [seqs + 1] on the device, ascending) attends the
- * tokens of its prompt up to itself, softmax of scale * q.k.  q and out are [tokens][heads][head_dim],
- * k and v [tokens][kv_heads][head_dim], heads a multiple of kv_heads; strides[0..7] are the token and
- * head strides, in elements, of q, k, v and out, whose rows start on 16 bytes.  dtype ENX_F16 or
- * ENX_BF16; head_dim a multiple of 8, at most 128.  Rows of no prompt are left as they were, and no
- * row depends on one it does not attend, whatever that holds.  Scores, softmax and sums in f32, weights
- * rounded to the dtype for their product with v.  No workspace.  enx_raw_check reports a bounded wait
- * that gave up. */
+ * (rows offsets[s] to offsets[s + 1] - 1; offsets int32 [seqs + 1] on the device, ascending) attends
+ * the tokens of its prompt up to itself, softmax of scale * q.k.  q and out are [tokens][heads]
+ * [head_dim], k and v [tokens][kv_heads][head_dim], heads a multiple of kv_heads; strides[0..7] are
+ * the token and head strides, in elements, of q, k, v and out, whose rows start on 16 bytes.  dtype
+ * ENX_F16 or ENX_BF16; head_dim a multiple of 8, at most 128; at most 2^24 tokens and 65536 prompts.
+ * Rows of no prompt are left as they were, and no row depends on one it does not attend, whatever
+ * that holds.  Scores, softmax and sums in f32, weights rounded to the dtype for their product with
+ * v.  No workspace.  enx_raw_check reports a bounded wait that gave up. */
 ENX_API enx_status enx_attn_packed(const void* q, const void* k, const void* v, void* out,
                                    const int64_t* strides, const int32_t* offsets, uint32_t seqs,
                                    uint32_t tokens, uint32_t heads, uint32_t kv_heads,

@@ -171,6 +171,18 @@ def test_rising_scores_and_wild_scales(gpu, dtype):
     check(q, out, [n], ks, vs, 0.3)
 
 
+@pytest.mark.parametrize("dtype,queries", [(F32, 1), (BF16, 2)])
+def test_more_sequences_than_threads_of_a_block(gpu, dtype, queries):
+    rng = np.random.default_rng(14)
+    lengths = [int(v) for v in rng.integers(0, 70, 300)]
+    lengths[:3], lengths[250] = [0, 0, 0], 700
+    table, pool, ks, vs = cache(rng, lengths, 1, 64, 16)
+    q = torch.from_numpy(rng.standard_normal((300, queries, 3, 64)).astype(np.float32)).to(dtype).cuda()
+    out = torch.full_like(q, 7.0)
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32(lengths), out, 1, 16)
+    check(q, out, lengths, ks, vs, 0.125)
+
+
 def test_padded_batch_strides_and_three_axes(gpu):
     rng = np.random.default_rng(5)
     lengths = [40, 0, 200]

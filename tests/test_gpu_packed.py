@@ -225,6 +225,36 @@ def test_prompt_then_pages_then_decode(gpu):
     assert float((far - 2.0 ** -9 * vv.double().abs().amax()).max()) <= 0 and status.item() == 0
 
 
+def test_a_wait_that_gives_up_is_reported(gpu):
+    q, k, v, ends = make([700, 90], 3, 1, 64, F16, 12)
+    out = torch.empty_like(q)
+    K.raw_check()
+    try:
+        K.set_wait_limit(1)  # one poll, which may be enough or not
+        K.attn_packed(q, k, v, out, ends)
+        try:
+            K.raw_check()
+            check(out, q, k, v, ends)
+        except EnxError as e:
+            assert e.status == 5
+    finally:
+        K.set_wait_limit(0)
+    K.attn_packed(q, k, v, out, ends)
+    K.raw_check()
+    check(out, q, k, v, ends)
+
+
+@pytest.mark.parametrize("prompts", [33, 300])
+def test_many_prompts(gpu, prompts):
+    """More than a warp of prompts, of all lengths, and empty ones between them."""
+    lengths = [(7 * i * i + 3 * i) % 290 for i in range(prompts)]
+    q, k, v, ends = make(lengths, 4, 2, 32, BF16, 13)
+    out = torch.full_like(q, 7.0)
+    K.attn_packed(q, k, v, out, ends)
+    K.raw_check()
+    check(out, q, k, v, ends)
+
+
 def test_refused_arguments(gpu):
     q, k, v, ends = make([9], 4, 2, 64, F16)
     ok = dict(q=q, k=k, v=v, out=torch.empty_like(q), offsets=ends)

@@ -161,7 +161,6 @@ __device__ __forceinline__ uint32_t rank_of(const Ranker& r, uint32_t flags, uin
 // last page that others hold as well is prepared by giving the row a copy of it.  All writers of
 // such a page take copies unless nobody else holds it: then the first of them in the list keeps it.
 // One CTA: the work is a few words per row, and everything hangs on the order of the list.
-// 5 us for 512 rows of a 9000-page pool.
 // Workspace: writers[pages], first[pages], found[pages], wanted[rows].
 __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const int32_t* __restrict__ list,
                                                            const int32_t* __restrict__ add, uint32_t n,

@@ -281,6 +281,36 @@ def test_write_grow_attend_in_one_captured_step(gpu):
     K.raw_check()
 
 
+def test_nothing_cached_yet_and_in_place_write(gpu):
+    rng = np.random.default_rng(15)
+    q = torch.from_numpy(rng.standard_normal((5, 1, 4, 64)).astype(np.float32)).cuda()
+    out = torch.full_like(q, 7.0)
+    pool = torch.full((3, K.kv4_page_bytes(16, 2, 64)), 0xFF, dtype=torch.uint8, device="cuda")
+    K.attn_kv4(q, pool, i32(np.full((5, 3), -1)), i32([0] * 5), out, 2, 16)
+    assert (out == 0).all()
+    k, v = rows(rng, (7, 2, 64), F16), rows(rng, (7, 2, 64), F16)
+    want = [twin.values(*twin.quantise(x.float().cpu().numpy())).astype(np.float16) for x in (k, v)]
+    K.kv4_write(k, v, pool, i32([[1]]), i32([0] * 7), i32(np.arange(7)), 16, k, v)  # the values replace their source
+    assert (k.cpu().numpy() == want[0]).all() and (v.cpu().numpy() == want[1]).all()
+
+
+def test_two_calls_at_once(gpu):
+    rng = np.random.default_rng(16)
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    work = []
+    for n in ([3000, 17, 900], [64] * 40):
+        table, pool, ks, vs = cache(rng, n, 1, 64, 32)
+        q = torch.from_numpy(rng.standard_normal((len(n), 1, 5, 64)).astype(np.float32)).cuda()
+        work.append((q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32(n), torch.zeros_like(q), n, ks, vs))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for side, (q, pool, table, lengths, out, *_) in zip(sides, work):
+            K.attn_kv4(q, pool, table, lengths, out, 1, 32, stream=side)
+    torch.cuda.synchronize()
+    for q, _, _, _, out, n, ks, vs in work:
+        check(q, out, n, ks, vs, 0.125)
+
+
 def test_another_stream(gpu):
     rng = np.random.default_rng(11)
     table, pool, ks, vs = cache(rng, [400, 90], 1, 64, 64)
@@ -341,7 +371,8 @@ def test_refused_arguments(gpu):
     for bad in (dict(q=q.double(), out=q.double()), dict(out=torch.zeros_like(q).half()), dict(pool=pool[:, :-16].contiguous()),
                 dict(table=t.long()), dict(lengths=i32([1])), dict(seqs=i32([0])), dict(page_tokens=8), dict(kv_heads=3),
                 dict(scale=0.0), dict(scale=math.nan), dict(workspace=torch.empty(16, dtype=torch.uint8, device="cuda")),
-                dict(q=q.transpose(2, 3).contiguous().transpose(2, 3)), dict(q=q.cpu()), dict(table=t[:1])):
+                dict(q=q.transpose(2, 3).contiguous().transpose(2, 3)), dict(q=q.cpu()), dict(table=t[:1]),
+                dict(out=torch.zeros(2 * 4 * 64 + 1, device="cuda")[1:].view(2, 1, 4, 64))):
         with pytest.raises((ValueError, EnxError)):
             K.attn_kv4(**{**ok, **bad})
     k = torch.zeros(2, 2, 64, device="cuda")

@@ -162,6 +162,29 @@ def test_nothing_to_do(gpu):
     check(out, q, k, v, ends)
 
 
+@pytest.mark.parametrize("t,heads,kv", [(1, 1, 1), (1, 4, 2), (3, 1, 1)])
+def test_the_smallest_tensors(gpu, t, heads, kv):
+    """Axes of one entry have no step of their own."""
+    q, k, v, ends = make([t], heads, kv, 64, BF16, 14)
+    out = torch.full_like(q, 7.0)
+    K.attn_packed(q, k, v, out, ends)
+    check(out, q, k, v, ends)
+
+
+def test_two_calls_at_once(gpu):
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    work = [make([900, 40, 300], 6, 2, hd, F16, 15 + hd) for hd in (64, 128)]
+    outs = [torch.zeros_like(w[0]) for w in work]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for side, (q, k, v, ends), out in zip(sides, work, outs):
+            K.attn_packed(q, k, v, out, ends, stream=side)
+    torch.cuda.synchronize()
+    K.raw_check()
+    for (q, k, v, ends), out in zip(work, outs):
+        check(out, q, k, v, ends)
+
+
 def test_captured_on_another_stream(gpu):
     q, k, v, ends = make([300, 500], 4, 2, 64, BF16, 8)
     out = torch.zeros_like(q)

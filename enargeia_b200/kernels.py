@@ -177,12 +177,14 @@ def _call_on(tensors, stream, name: str, *args) -> None:
 
 
 def _enough(workspace: Optional[torch.Tensor], nbytes: int, like: torch.Tensor, stream) -> torch.Tensor:
-    """The caller's workspace, or one for this call, whose memory is not handed out before it is done."""
+    """The caller's workspace, or one for this call from the memory of the stream that it runs on (the
+    allocator orders a block's users by the stream that it was taken on)."""
     if workspace is None:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-        if stream is not None:
-            workspace.record_stream(stream)
-    elif workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous() or not workspace.is_cuda:
+        if stream is None:
+            return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    if workspace.numel() * workspace.element_size() < nbytes or not workspace.is_contiguous() or not workspace.is_cuda:
         raise ValueError(f"the workspace has to have {nbytes} contiguous bytes on the device")
     return workspace
 

@@ -277,7 +277,8 @@ ENX_API enx_status enx_pages_compact(const int32_t* table, const int32_t* length
                                      int32_t* count, int32_t* status, const enx_pages_dims* dims,
                                      void* workspace, void* stream);
 /* Copies page pairs[i][0] onto page pairs[i][1] in every layer of pool [layers][pages][page_bytes]
- * for the first min(count[0], capacity) pairs.  No page may be source and destination of one call,
+ * for the first min(count[0], capacity) pairs (a count outside 0 .. capacity raises
+ * ENX_PAGES_BAD_PAGE too).  No page may be source and destination of one call,
  * nor a destination twice (the calls above make no such pairs).  page_bytes a multiple of 16, the
  * pool 16-byte aligned. */
 ENX_API enx_status enx_pages_copy(void* pool, uint32_t layers, uint32_t pages, uint32_t page_bytes,

@@ -281,6 +281,28 @@ def test_write_grow_attend_in_one_captured_step(gpu):
     K.raw_check()
 
 
+def test_a_workspace_is_taken_on_the_stream_of_the_call(gpu):
+    """A block that the current stream has just given back, and still works on, is not this call's
+    workspace on another stream."""
+    rng = np.random.default_rng(17)
+    table, pool, ks, vs = cache(rng, [2000], 1, 64, 64)
+    q = torch.from_numpy(rng.standard_normal((1, 1, 4, 64)).astype(np.float32)).cuda()
+    dev, out, t, n = torch.from_numpy(pool.bytes).cuda(), torch.zeros_like(q), i32(table), i32([2000])
+    side, size = torch.cuda.Stream(), K._lib.load().enx_attn_kv4_workspace_bytes(1, 64)
+    torch.cuda.synchronize()
+    busy = torch.empty(size, dtype=torch.uint8, device="cuda")
+    at = busy.data_ptr()
+    torch.cuda._sleep(20_000_000)
+    busy.fill_(0xFF)  # queued behind the sleep
+    del busy
+    ws = K._enough(None, size, q, side)
+    assert ws.data_ptr() != at
+    del ws
+    K.attn_kv4(q, dev, t, n, out, 1, 64, stream=side)
+    torch.cuda.synchronize()
+    check(q, out, [2000], ks, vs, 0.125)
+
+
 def test_nothing_cached_yet_and_in_place_write(gpu):
     rng = np.random.default_rng(15)
     q = torch.from_numpy(rng.standard_normal((5, 1, 4, 64)).astype(np.float32)).cuda()

@@ -294,6 +294,10 @@ __device__ __forceinline__ uint32_t kv_head_of(const AttnArgs& a, uint32_t part)
 
 __device__ __forceinline__ uint32_t chunks_of(uint32_t len) { return (len + kKvChunk - 1) / kKvChunk; }
 
+// What a head of a sequence counts in the split of the work: its chunks, and one for its beginning and end
+// (operands of q, reductions, results), which cost about as much as a chunk.
+__device__ __forceinline__ uint32_t share_of(uint32_t len) { return len ? chunks_of(len) + 1 : 0; }
+
 // Table row and length of batch entry b; row -1: not to be computed.
 __device__ __forceinline__ void sequence(const AttnArgs& a, uint32_t b, int32_t* row, uint32_t* len) {
     int32_t r = a.seqs ? a.seqs[b] : (int32_t)b;
@@ -329,8 +333,8 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 
 }  // namespace
 
-// The work is the list of all (sequence, kv head, row tile, chunk of 64 tokens), in that order; each
-// warp takes an equal run of it, whatever the lengths, and hands on partial results for the (at most
+// The work is the list of all (sequence, kv head, row tile, chunk of 64 tokens), in that order, with one
+// more place for each head's beginning and end; each warp takes an equal run of it, whatever the lengths, and hands on partial results for the (at most
 // two) heads that it shares with its neighbours; k_kv4_join adds those up.  A row tile is 8 NT of the
 // kv head's queries * (heads / kv_heads) query rows.  Warps have nothing to do with one another (with
 // four of them on one head, joining their sums cost as much as a 1000-token head itself).
@@ -357,8 +361,8 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 // half a step 2^-11, before a sum that is rounded to 16 bits anyway).
 //
 // Bound: 4.5 bits a value leave two to three instructions a value at full HBM rate, and the loop needs about
-// three (256 sequences up to 2048 tokens, 14/2 heads of 64, f32: 32 us, 1.2 TB/s, a quarter of it at the heads'
-// ends; four up to 131072, 32/8 heads of 128, bf16: 104 us, 4.2 TB/s; ALU pipe 40 to 50 % busy, issue 55 to 60 %);
+// three (256 sequences up to 2048 tokens, 14/2 heads of 64, f32: 30 us, 1.3 TB/s, a quarter of it at the heads'
+// ends; 32 us without their place in the split; four up to 131072, 32/8 heads of 128, bf16: 105 us, 4.2 TB/s; ALU pipe 40 to 50 % busy, issue 55 to 60 %);
 // tcgen05 would want the codes widened into shared memory first, which costs more than
 // the products do on mma.sync at 8 rows.
 template <typename T, int HD, int NT, bool SPLIT>
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
         int32_t row;
         uint32_t len;
         sequence(a, b, &row, &len);
-        mine += chunks_of(len) * parts;
+        mine += share_of(len) * parts;
     }
     uint32_t incl = mine;
 #pragma unroll
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
             uint32_t len;
             sequence(a, b, &row, &len);
             a.head_ws[b] = at;
-            at += chunks_of(len) * parts;
+            at += share_of(len) * parts;
         }
         if (tid == 0) {
             a.head_ws[a.batch] = total;
@@ -426,8 +430,8 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
     __syncthreads();
     const uint32_t run = warp * gridDim.x + blockIdx.x;  // neighbouring runs on different SMs
     const unsigned long long first = (unsigned long long)run * per;
-    const uint32_t u0 = (uint32_t)min((unsigned long long)total, first), u1 = min(total, u0 + per), units = u1 - u0;
-    if (units == 0) return;
+    const uint32_t u0 = (uint32_t)min((unsigned long long)total, first), u1 = min(total, u0 + per);
+    if (u0 == u1) return;
     Cursor c{0, 0, 0, 0, -1};
     {
         uint32_t lower = 0;  // threads whose sequences begin at or before u0
@@ -438,13 +442,37 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
         for (;; ++c.b) {
             if (c.b >= a.batch) return;  // (only if the lengths change under the call)
             sequence(a, c.b, &c.row, &c.len);
-            const uint32_t n = chunks_of(c.len) * parts;
+            const uint32_t n = share_of(c.len) * parts;
             if (u0 < at + n) break;
             at += n;
         }
-        c.part = (u0 - at) / chunks_of(c.len);
-        c.chunk = (u0 - at) % chunks_of(c.len);
+        // place 0 of a head's share is its beginning, place i chunk i - 1
+        c.part = (u0 - at) / share_of(c.len);
+        c.chunk = (u0 - at) % share_of(c.len);
     }
+    // the chunks among the run's units: a beginning at its end is left to the next run
+    uint32_t units = 0;
+    {
+        Cursor head = c;
+        uint32_t left = u1 - u0, place = c.chunk;
+        while (left) {
+            if (place == 0) {
+                --left;
+                place = 1;
+            }
+            const uint32_t take = min(left, share_of(head.len) - place);
+            units += take;
+            left -= take;
+            if (left) {
+                head.chunk = chunks_of(head.len) - 1;
+                advance(a, head, parts);
+                if (head.b >= a.batch) break;
+                place = 0;
+            }
+        }
+        c.chunk = c.chunk ? c.chunk - 1 : 0;
+    }
+    if (units == 0) return;
 
     // ---- feeding: lane i copies the i-th page of a chunk, or section i of a half page of 128 --------
     const uint32_t limit = g_kv4_spin;
@@ -909,16 +937,16 @@ __global__ void __launch_bounds__(256) k_kv4_join(AttnArgs a) {
     uint32_t len;
     sequence(a, b, &row, &len);
     if (row < 0) return;
-    const uint32_t per = a.head_ws[a.batch + 1], n = chunks_of(len);
-    const uint32_t u0 = a.head_ws[b] + part * n, u1 = u0 + n;
-    const uint32_t c0 = u0 / per, c1 = len ? (u1 - 1) / per : c0 + 1;
+    const uint32_t per = a.head_ws[a.batch + 1], n = share_of(len);
+    const uint32_t u0 = a.head_ws[b] + part * n;  // the head's beginning; its chunks follow
+    const uint32_t c0 = (u0 + 1) / per, c1 = len ? (u0 + n - 1) / per : c0 + 1;
     if (c0 == c1) return;  // one run had it all
     const uint32_t kvh = part / a.tiles, d4 = tid % kLanes, local = tid / kLanes % COLS, share = tid / kLanes / COLS;
     const uint32_t col = blockIdx.y * COLS + local, r = part % a.tiles * kCols + col;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float ls = 0.f;
     if (len) {
-        // run c's piece begins at its own first unit (slot 0) or, only for c0, behind it (slot 1)
+        // run c's piece is the first of the run (slot 0) or, only for c0, comes behind another head's (slot 1)
         auto piece = [&](uint32_t c) {
             return a.part + ((size_t)(2 * c + (u0 > c * per ? 1 : 0)) * kCols + col) * (HD + 4);
         };
@@ -1096,7 +1124,7 @@ extern "C" enx_status enx_attn_kv4(const void* q, const int64_t* strides, const 
     if (rows > 65536 || (uint64_t)batch * queries * heads > 0x7fffffffull)
         return fail(ENX_ERR_RANGE, "enx_attn_kv4: too many query rows for one call");
     const uint32_t nt = rows <= 8 ? 1 : 2, tiles = (uint32_t)((rows + 8 * nt - 1) / (8 * nt));
-    const uint64_t chunks = ((uint64_t)d->width * d->page_tokens + kKvChunk - 1) / kKvChunk;
+    const uint64_t chunks = ((uint64_t)d->width * d->page_tokens + kKvChunk - 1) / kKvChunk + 1;  // and a head's beginning
     if ((uint64_t)batch * d->kv_heads * tiles > 0x7fffffffull / chunks)
         return fail(ENX_ERR_RANGE, "enx_attn_kv4: batch x table width is too large for one call");
     const uint64_t units = (uint64_t)batch * d->kv_heads * tiles * chunks;

@@ -161,61 +161,61 @@ __device__ __forceinline__ uint32_t rank_of(const Ranker& r, uint32_t flags, uin
 // last page that others hold as well is prepared by giving the row a copy of it.  All writers of
 // such a page take copies unless nobody else holds it: then the first of them in the list keeps it.
 // One CTA: the work is a few words per row, and everything hangs on the order of the list.
-// Workspace: writers[pages], first[pages], found[pages], wanted[rows].
+// Every row's chain of reads (list, length, table, count) is gone through once and kept in the workspace: each
+// further step of it costs more than all the arithmetic.  A thread hands out a row's pages, a warp where there
+// are more than kPgFew.  512 rows that each copy or take a page: 10 us (19 with a warp a row and the chains repeated).
+// Workspace: writers[pages], first[pages], found[pages], then per row wanted (64 bits), its last page if that
+// is shared and about to be written (or -1), and its length.
+constexpr uint32_t kPgFew = 4;
+
 __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const int32_t* __restrict__ list,
                                                            const int32_t* __restrict__ add, uint32_t n,
                                                            int32_t* __restrict__ pairs, int32_t* __restrict__ count,
                                                            int32_t* ws) {
     extern __shared__ uint32_t seen[];
-    __shared__ int s_bad;
+    __shared__ int s_bad, s_many;
     __shared__ unsigned long long s_sum[32], s_run;
     __shared__ Ranker ranks;
     int32_t *writers = ws, *first = ws + a.pages, *found = ws + 2 * (size_t)a.pages;
     unsigned long long* wanted = reinterpret_cast<unsigned long long*>(ws + 3 * (size_t)a.pages + (a.pages & 1));
+    int32_t* last = reinterpret_cast<int32_t*>(wanted + a.rows);
+    uint32_t* lens = reinterpret_cast<uint32_t*>(last + a.rows);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pt = a.page_tokens;
     for (uint32_t i = tid; i < (a.rows + 31) / 32; i += kPgThreads) seen[i] = 0;
     if (tid == 0) {
-        s_bad = 0;
+        s_bad = s_many = 0;
         s_run = 0;
         count[0] = count[1] = 0;
     }
     __syncthreads();
-    // per row: its last page if that is partly filled, held by others too and about to be written
-    auto shared_last = [&](int32_t row, uint32_t more, uint32_t* len) -> int32_t {
-        *len = (uint32_t)a.lengths[row];
-        if (!more || *len % pt == 0) return -1;
-        const int32_t p = a.table[(size_t)row * a.width + *len / pt];
-        return a.refs[p] > 1 ? p : -1;
-    };
     for (uint32_t i = tid; i < n; i += kPgThreads) {
         const int32_t row = list[i], more = add[i];
         bool ok = claim_row(seen, row, a.rows) && more >= 0;
+        int32_t shared = -1, len = 0;
         if (ok) {
-            const int32_t len = a.lengths[row];
+            len = a.lengths[row];
             ok = len >= 0 && (unsigned long long)len + (uint32_t)more <= (unsigned long long)a.width * pt;
             if (ok && more && len % pt) {
                 const int32_t p = a.table[(size_t)row * a.width + len / pt];
                 ok = p >= 0 && (uint32_t)p < a.pages;
+                if (ok && a.refs[p] > 1) {
+                    shared = p;
+                    writers[p] = 0;
+                    first[p] = 0x7fffffff;
+                }
             }
         }
         if (!ok) s_bad = 1;
+        last[i] = shared;
+        lens[i] = (uint32_t)len;
     }
     __syncthreads();
     if (s_bad) {
         if (tid == 0) atomicOr(a.status, kPgBadList);
         return;
     }
-    uint32_t len;
     for (uint32_t i = tid; i < n; i += kPgThreads) {
-        const int32_t p = shared_last(list[i], (uint32_t)add[i], &len);
-        if (p >= 0) {
-            atomicExch(&writers[p], 0);
-            atomicExch(&first[p], 0x7fffffff);
-        }
-    }
-    __syncthreads();
-    for (uint32_t i = tid; i < n; i += kPgThreads) {
-        const int32_t p = shared_last(list[i], (uint32_t)add[i], &len);
+        const int32_t p = last[i];
         if (p >= 0) {
             atomicAdd(&writers[p], 1);
             atomicMin(&first[p], (int32_t)i);
@@ -227,9 +227,10 @@ __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const in
         const uint32_t i = i0 + tid;
         unsigned long long mine = 0;
         if (i < n) {
-            const int32_t p = shared_last(list[i], (uint32_t)add[i], &len);
-            const bool copy = p >= 0 && !(atomicAdd(&writers[p], 0) == a.refs[p] && atomicAdd(&first[p], 0) == (int32_t)i);
-            const uint32_t fresh = pages_of(len + (uint32_t)add[i], pt) - pages_of(len, pt);
+            const int32_t p = last[i];
+            const bool copy = p >= 0 && !(__ldcg(&writers[p]) == a.refs[p] && __ldcg(&first[p]) == (int32_t)i);
+            const uint32_t fresh = pages_of(lens[i] + (uint32_t)add[i], pt) - pages_of(lens[i], pt);
+            if (fresh > kPgFew) s_many = 1;
             mine = ((unsigned long long)copy << 32) + fresh + copy;
         }
         unsigned long long incl = mine;
@@ -270,30 +271,40 @@ __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const in
         return;
     }
     __syncthreads();
-    // a warp per row hands its pages out
-    for (uint32_t i = warp; i < n; i += kPgThreads / 32) {
+    // the pages behind a row's copy: fresh ones from page `at` of the found ones on
+    auto take = [&](int32_t* entries, uint32_t held, uint32_t at, uint32_t k) {
+        const int32_t to = found[at + k];
+        entries[held + k] = to;
+        a.refs[to] = 1;
+    };
+    for (uint32_t i = tid; i < n; i += kPgThreads) {
         const int32_t row = list[i];
-        const uint32_t more = (uint32_t)add[i], old = (uint32_t)a.lengths[row];
+        const uint32_t old = lens[i], held = pages_of(old, pt);
         const unsigned long long at = wanted[i], next = i + 1 < n ? wanted[i + 1] : s_run;
         const uint32_t at_page = (uint32_t)at, copy = (uint32_t)(next >> 32) - (uint32_t)(at >> 32);
         const uint32_t fresh = (uint32_t)next - at_page - copy;
         int32_t* entries = a.table + (size_t)row * a.width;
-        if (copy && lane == 0) {
-            const int32_t from = entries[old / pt], to = found[at_page];
+        if (copy) {
+            const int32_t from = last[i], to = found[at_page];
             entries[old / pt] = to;
             a.refs[to] = 1;
             atomicSub(&a.refs[from], 1);
             pairs[2 * (at >> 32)] = from;
             pairs[2 * (at >> 32) + 1] = to;
         }
-        for (uint32_t k = lane; k < fresh; k += 32) {
-            const int32_t to = found[at_page + copy + k];
-            entries[pages_of(old, pt) + k] = to;
-            a.refs[to] = 1;
-        }
-        __syncwarp();
-        if (lane == 0) a.lengths[row] = (int32_t)(old + more);
+        if (fresh <= kPgFew)
+            for (uint32_t k = 0; k < fresh; ++k) take(entries, held, at_page + copy, k);
+        a.lengths[row] = (int32_t)(old + (uint32_t)add[i]);
     }
+    if (s_many)
+        for (uint32_t i = warp; i < n; i += kPgThreads / 32) {
+            const unsigned long long at = wanted[i], next = i + 1 < n ? wanted[i + 1] : s_run;
+            const uint32_t at_page = (uint32_t)at, copy = (uint32_t)(next >> 32) - (uint32_t)(at >> 32);
+            const uint32_t fresh = (uint32_t)next - at_page - copy;
+            if (fresh > kPgFew)
+                for (uint32_t k = lane; k < fresh; k += 32)
+                    take(a.table + (size_t)list[i] * a.width, pages_of(lens[i], pt), at_page + copy, k);
+        }
     if (tid == 0) {
         count[0] = (int32_t)copies;
         count[1] = (int32_t)total;
@@ -470,7 +481,7 @@ static enx_status pages_rows(const PagesArgs& a, const int32_t* list, const int3
 }
 
 extern "C" size_t enx_pages_workspace_bytes(uint32_t rows, uint32_t pages) {
-    return 4 * (size_t)pages * sizeof(int32_t) + (size_t)rows * 8 + 16;
+    return 4 * (size_t)pages * sizeof(int32_t) + (size_t)rows * 16 + 16;
 }
 
 extern "C" enx_status enx_pages_free(int32_t* table, int32_t* lengths, int32_t* refs, const int32_t* rows,

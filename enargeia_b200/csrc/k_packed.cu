@@ -262,11 +262,13 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
 
 // 2^x for two x <= 9: x = n + f with n the nearest whole number (the low bits of x + 1.5 * 2^23),
 // 2^f by the cubic with the least relative error on [-1/2, 1/2] (Remez exchange: 7.5e-5, below the
-// weights' rounding to 16 bits), n added to its exponent.  x is cut at -126, where 2^x counts for nothing.
+// weights' rounding to 16 bits), n added to its exponent.  Below 2^-127 that sum would be negative, and is cut
+// to 0: what a row does not see (x = -inf) has no weight at all.  (bf16 has 2^-126 as a normal number, and
+// times a V element of 1e38 it counts.)  x is cut at -250 first, so that n stays in the word.
 __device__ __forceinline__ void ex2_poly(Pair xy, float& a, float& b) {
     float x, y;
     unpair(xy, x, y);
-    xy = pair(fmaxf(x, -126.f), fmaxf(y, -126.f));
+    xy = pair(fmaxf(x, -250.f), fmaxf(y, -250.f));
     const Pair big = pair(12582912.f, 12582912.f), nbig = pair(-12582912.f, -12582912.f), one = pair(-1.f, -1.f);
     const Pair n = add2(xy, big);
     const Pair f = fma2(add2(n, nbig), one, xy);
@@ -276,8 +278,8 @@ __device__ __forceinline__ void ex2_poly(Pair xy, float& a, float& b) {
     float nx, ny;
     unpair(n, nx, ny);
     unpair(r, a, b);
-    a = __int_as_float(__float_as_int(a) + (__float_as_int(nx) << 23));
-    b = __int_as_float(__float_as_int(b) + (__float_as_int(ny) << 23));
+    a = __int_as_float(max(__float_as_int(a) + (__float_as_int(nx) << 23), 0));
+    b = __int_as_float(max(__float_as_int(b) + (__float_as_int(ny) << 23), 0));
 }
 
 // Rows [begin, begin + len) of the packed tensors, the pair-th 256 of them, of one head; len 0: no more.

@@ -295,3 +295,41 @@ def test_refused_arguments(gpu):
     thin = torch.empty(9, 2, 12, dtype=F16, device="cuda")
     with pytest.raises(EnxError):
         K.attn_packed(thin, thin, thin, torch.empty_like(thin), ends)
+
+
+@pytest.mark.parametrize("hd,dtype,big", [(128, BF16, 3e38), (128, BF16, 1e30), (72, BF16, 3e38), (64, BF16, 3e38), (128, F16, 6e4),
+                                          (64, F16, 6e4)])
+def test_large_values_that_a_row_does_not_see_do_not_reach_it(gpu, hd, dtype, big):
+    """Finite ones: a weight of what a row does not see is zero, not merely small."""
+    lengths = [130, 300, 40]
+    q, k, v, ends = make(lengths, 2, 1, hd, dtype, 16, spare=90)
+    clean = torch.empty_like(q)
+    K.attn_packed(q, k, v, clean, ends)
+    signs = 1 - 2 * (torch.arange(v.numel(), device="cuda").reshape(v.shape) % 3 % 2)
+    loud = (big * signs).to(dtype)
+    v2, k2, q2 = v.clone(), k.clone(), q.clone()
+    v2[130 + 200:430], k2[130 + 200:430] = loud[330:430], loud[330:430]  # the second prompt's later tokens, its diagonal tiles
+    v2[430:], k2[430:], q2[430:] = loud[430:], loud[430:], loud[430:]    # the third prompt, and rows of none
+    out = torch.empty_like(q)
+    K.attn_packed(q2, k2, v2, out, ends)
+    assert torch.equal(out[:130], clean[:130]) and torch.equal(out[130:330], clean[130:330])
+    # every token's own successor is loud: what a row sees of the rest of its tile is what it saw before
+    for at in (1, 5, 63, 64, 127):
+        v2, k2 = v.clone(), k.clone()
+        v2[130 + at:430] = loud[130 + at:430]
+        K.attn_packed(q, k2, v2, out, ends)
+        assert torch.equal(out[130:130 + at], clean[130:130 + at]), at
+
+
+@pytest.mark.parametrize("hd,dtype,big", [(128, BF16, 3e38), (64, BF16, 3e38), (128, F16, 6e4)])
+def test_a_weight_that_underflows_is_zero(gpu, hd, dtype, big):
+    """Four tokens lie some 500 below the others in the exponent of two: whatever they hold, they add nothing."""
+    q, k, v, ends = make([400], 2, 1, hd, dtype, 17)
+    q = q.abs()
+    k[:4] = -45 * 128 / hd
+    quiet, loud = torch.empty_like(q), torch.empty_like(q)
+    v[:4] = 0
+    K.attn_packed(q, k, v, quiet, ends)
+    v[:4] = big
+    K.attn_packed(q, k, v, loud, ends)
+    assert torch.equal(quiet[4:], loud[4:]) and (loud[0] == v[0]).all()

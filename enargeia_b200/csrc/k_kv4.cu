@@ -278,6 +278,16 @@ __device__ __forceinline__ void codes_of(uint32_t x, uint32_t& lo, uint32_t& hi)
 // 2^e, for e within the range of normal floats
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 
+// log2 of a V scale's size, as the choice of a unit for the weights takes it: 2^-25 and less count as 2^-25
+__device__ __forceinline__ float log2_scale(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fminf(fmaxf(x, 0x1p-25f), 65504.f)));
+    return y;
+}
+
+// 2^x of a whole number x within the range of normal floats
+__device__ __forceinline__ float pow2_whole(float x) { return __int_as_float(__float_as_int(x + (12582912.f + 127.f)) << 23); }
+
 // x's exponent, cut to a range in which pow2f of it, its negative and small sums are normal
 __device__ __forceinline__ int exponent_of(float x) {
     const int e = (int)((__float_as_uint(x) >> 23) & 0xFF) - 127;
@@ -351,6 +361,10 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 //   tiles need no maximum across lanes (one vote); p stays below 2^8.
 //   O^T [dim][row] += V codes^T (A) * w (B), w = p * scale, which one movmatrix per 8x8 turns from
 //   the accumulator's layout into the operand's.  p * offset is summed apart, in f32 FMAs.
+//   w goes in as f16 in units of a power of two of the row's and the group's own, in which the largest w
+//   met so far is 16 to 32: a token with a large scale that this row gives no weight to, or the other
+//   group's scales, must not take the bits of those that count.  The vote that guards m guards them too.  (A
+//   token whose V is nothing but zeros counts as one of scale 2^-25; beside it what lies 2^-50 below is lost.)
 //
 // With f32 rows (SPLIT) q and w go in as two f16 each, high and remainder, so that products are good
 // to 2^-22.  mma.sync aligns products by their operands' exponents, of which a subnormal's is above
@@ -365,8 +379,9 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 // ends; 32 us without their place in the split; four up to 131072, 32/8 heads of 128, bf16: 105 us, 4.2 TB/s; ALU pipe 40 to 50 % busy, issue 55 to 60 %);
 // tcgen05 would want the codes widened into shared memory first, which costs more than
 // the products do on mma.sync at 8 rows.
+// Three CTAs an SM where their 168 registers suffice: left to itself the compiler takes 182 to 189 and two.
 template <typename T, int HD, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
+__global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ? 3 : 2) k_kv4_attn(AttnArgs a) {
     constexpr uint32_t G = HD > 64 ? HD / 64 : 1;         // groups of a row
     constexpr uint32_t W = HD / G / 8;                    // words of a group's codes: 8 (hd 32: 4)
     constexpr uint32_t KW = W / 4;                        // K words a lane takes of a group
@@ -539,7 +554,8 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
     uint32_t qf[NT][G * KW * 2][2], ql[SPLIT ? NT : 1][SPLIT ? G * KW * 2 : 1][2];
     float kfac[NT][2], qsum[NT][2][G];
     int32_t last[NT][2];  // the last token a column sees
-    float m[NT][2], l[NT][2], o[NT][MT][4], om[NT][2][G], fv = 0.f;
+    // m: a row's reference, lu: log2 of the unit of its weights in each group, whole numbers both
+    float m[NT][2], l[NT][2], o[NT][MT][4], om[NT][2][G], lu[NT][2][G];
 
     uint32_t begun = 0;  // the unit of the run with which the present head began
     bool gave_up = false;
@@ -618,7 +634,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
                     m[n][j] = kKvLow;
                     l[n][j] = 0.f;
 #pragma unroll
-                    for (uint32_t gr = 0; gr < G; ++gr) om[n][j][gr] = 0.f;
+                    for (uint32_t gr = 0; gr < G; ++gr) om[n][j][gr] = lu[n][j][gr] = 0.f;
                 }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -626,7 +642,6 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
                 for (uint32_t d = 0; d < MT; ++d)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[n][d][e] = 0.f;
-            fv = 0.f;
         }
 
         const uint32_t s = i % kKvStages;
@@ -653,7 +668,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
             auto hidden = [&](int p, int n, int e) {
                 return kEdge && (int32_t)(chunk0 + tok + 16 * p + (e < 2 ? kt0 : kt1)) > last[n][e & 1];
             };
-            float vtop = 0.f;
+            float vtop[G] = {};  // the largest scale of this lane's tokens
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const uint32_t at = tok + 16 * p, in_page = at & (stage_page - 1);
@@ -722,42 +737,64 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
                     }
                 }
 #pragma unroll
-                for (uint32_t gr = 0; gr < G; ++gr) vtop = fmaxf(vtop, fmaxf(v0[p][gr].x, v1[p][gr].x));
+                for (uint32_t gr = 0; gr < G; ++gr) vtop[gr] = fmaxf(vtop[gr], fmaxf(fabsf(v0[p][gr].x), fabsf(v1[p][gr].x)));
             }
-            bool over = vtop * fv > 64.f || fv == 0.f;
+            // a weight scale * 2^(s - m + lu) has to stay below 2^16, and s - m below 8
+            float room[G];
+#pragma unroll
+            for (uint32_t gr = 0; gr < G; ++gr) room[gr] = 15.5f - log2_scale(vtop[gr]);
+            bool over = false;
             float tops[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     tops[n][j] = fmaxf(fmaxf(sc[0][n][j], sc[0][n][2 + j]), fmaxf(sc[1][n][j], sc[1][n][2 + j]));
-                    over = over || tops[n][j] > m[n][j] + 8.f;
+#pragma unroll
+                    for (uint32_t gr = 0; gr < G; ++gr)
+                        over = over || tops[n][j] - m[n][j] > fminf(8.f, room[gr] - lu[n][j][gr]);
                 }
             if (__any_sync(0xffffffffu, over)) {
-                // new references: the rows' maxima, and a power of two that brings w to about 16
-                vtop = warp_max(vtop);
-                const float fv_new = vtop * fv > 64.f || fv == 0.f ? pow2f(3 - exponent_of(vtop)) : fv;
-                const float fo = fv == 0.f ? 1.f : fv_new / fv;
-                fv = fv_new;
+                // New references: the rows' maxima.  New units: the largest weight so far comes to 16 to 32 (what the
+                // unit says of the earlier ones, less what the reference's move takes off, or this tile's).
+                float lv[2][2][G];
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (uint32_t gr = 0; gr < G; ++gr) {
+                        lv[p][0][gr] = log2_scale(fabsf(v0[p][gr].x));
+                        lv[p][1][gr] = log2_scale(fabsf(v1[p][gr].x));
+                    }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float f[2];
+                    float f[G][2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float top = tops[n][j];
+                        float top = tops[n][j], wide[G];
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        top = fmaxf(top, m[n][j]);
-                        f[j] = ex2(m[n][j] - top);
+                        top = fmaxf(floorf(top), m[n][j]);
+                        const float moved = top - m[n][j], fm = ex2(-moved);
                         m[n][j] = top;
-                        l[n][j] *= f[j];
+                        l[n][j] *= fm;
 #pragma unroll
-                        for (uint32_t gr = 0; gr < G; ++gr) om[n][j][gr] *= f[j];
+                        for (uint32_t gr = 0; gr < G; ++gr) {
+                            wide[gr] = -INFINITY;
+#pragma unroll
+                            for (int p = 0; p < 2; ++p)
+                                wide[gr] = fmaxf(wide[gr], fmaxf(sc[p][n][j] - top + lv[p][0][gr], sc[p][n][2 + j] - top + lv[p][1][gr]));
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) wide[gr] = fmaxf(wide[gr], __shfl_xor_sync(0xffffffffu, wide[gr], x));
+                            const float unit = 4.f - fmaxf(floorf(wide[gr]), 4.f - lu[n][j][gr] - moved);
+                            f[gr][j] = fm * pow2_whole(unit - lu[n][j][gr]);
+                            lu[n][j][gr] = unit;
+                            om[n][j][gr] *= fm;
+                        }
                     }
 #pragma unroll
                     for (uint32_t d = 0; d < MT; ++d)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n][d][e] *= f[e & 1] * fo;
+                        for (int e = 0; e < 4; ++e) o[n][d][e] *= f[G == 1 ? 0 : d / 4][e & 1];
                 }
             }
 #pragma unroll
@@ -774,14 +811,19 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
 #pragma unroll
             for (uint32_t gr = 0; gr < G; ++gr) {
                 uint32_t wb[2][NT][2], wl[2][NT][2];
+                float unit[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) unit[n][j] = pow2_whole(lu[n][j][gr]);
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    const float s0 = v0[p][gr].x * fv, s1 = v1[p][gr].x * fv;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         float x[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = hidden(p, n, e) ? 0.f : sc[p][n][e] * (e < 2 ? s0 : s1);
+                        for (int e = 0; e < 4; ++e)
+                            x[e] = hidden(p, n, e) ? 0.f : sc[p][n][e] * ((e < 2 ? v0 : v1)[p][gr].x * unit[n][e & 1]);
                         const uint32_t h0 = pack_h2(x[0], x[1]), h1 = pack_h2(x[2], x[3]);
                         wb[p][n][0] = transpose8x8(h0);
                         wb[p][n][1] = transpose8x8(h1);
@@ -854,7 +896,6 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
         const bool head_done = c.chunk + 1 == chunks_of(c.len);
         if (head_done || i + 1 == units) {
             // ---- the head's result, or this run's part of it --------------------------------------------
-            const float back = fv == 0.f ? 0.f : kUp / fv;
             const uint32_t kvh = kv_head_of(a, c.part), tile = c.part - kvh * a.tiles;
             const bool whole = head_done && i - begun == c.chunk;
             // the run's first head goes to slot 0 of its two, one that began later to slot 1
@@ -863,9 +904,12 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float lt = l[n][j], mt[G];
+                    float lt = l[n][j], mt[G], back[G];
 #pragma unroll
-                    for (uint32_t gr = 0; gr < G; ++gr) mt[gr] = om[n][j][gr];
+                    for (uint32_t gr = 0; gr < G; ++gr) {
+                        mt[gr] = om[n][j][gr];
+                        back[gr] = kUp * pow2_whole(-lu[n][j][gr]);
+                    }
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) {
                         lt += __shfl_xor_sync(0xffffffffu, lt, x);
@@ -885,8 +929,8 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
                             float v[8];
 #pragma unroll
                             for (int d = 0; d < 4; ++d) {
-                                v[2 * d] = fmaf(o[n][gr * 4 + d][j], back, mt[gr]) * inv;
-                                v[2 * d + 1] = fmaf(o[n][gr * 4 + d][2 + j], back * kOdd, mt[gr]) * inv;
+                                v[2 * d] = fmaf(o[n][gr * 4 + d][j], back[gr], mt[gr]) * inv;
+                                v[2 * d + 1] = fmaf(o[n][gr * 4 + d][2 + j], back[gr] * kOdd, mt[gr]) * inv;
                             }
                             if (whole)
                                 store8(dst + gr * 64 + g * 8, v);
@@ -896,7 +940,7 @@ __global__ void __launch_bounds__(kKvWarps * 32) k_kv4_attn(AttnArgs a) {
                     } else {
 #pragma unroll
                         for (uint32_t d = 0; d < MT; ++d) {
-                            const float x0 = fmaf(o[n][d][j], back, mt[0]) * inv, x1 = fmaf(o[n][d][2 + j], back * kOdd, mt[0]) * inv;
+                            const float x0 = fmaf(o[n][d][j], back[0], mt[0]) * inv, x1 = fmaf(o[n][d][2 + j], back[0] * kOdd, mt[0]) * inv;
                             if (whole) {
                                 dst[g * 4 + 2 * d] = from_f<T>(x0);
                                 dst[g * 4 + 2 * d + 1] = from_f<T>(x1);

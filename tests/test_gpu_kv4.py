@@ -403,3 +403,55 @@ def test_refused_arguments(gpu):
                 dict(k=k[:, :, :63], v=k[:, :, :63]), dict(pool=pool[None]), dict(k_out=torch.zeros(2, 64, 2, device="cuda").mT)):
         with pytest.raises((ValueError, EnxError)):
             K.kv4_write(**{**good, **bad})
+
+
+def uneven(case, rng, n, hd):
+    """(K, V, q [2 heads, hd]) where V's scales lie up to eight powers of ten apart, between tokens that
+    one head or the other weighs, or between the groups of a row.  q is positive for head 0 and negative for head 1."""
+    q = np.abs(rng.standard_normal((2, hd))) + 0.1
+    q[1] *= -1
+    k, v = 0.1 * rng.standard_normal((n, 1, hd)), rng.standard_normal((n, 1, hd))
+    away = 60 / (np.abs(q).sum(1).min() * hd ** -0.5)  # K of one sign and this size: scores of about +-60
+    if case == "early":
+        v *= 3e-5
+        k[5], v[5] = -away, 5e8 * v[5]
+    elif case == "late":
+        v *= 3e-5
+        k[n - 9], v[n - 9] = -away, 5e8 * v[n - 9]
+    elif case == "groups":  # of hd 128: the first half of a row large, the other small
+        v[..., :64] *= 3e3
+        v[..., 64:] *= 3e-4
+    elif case == "rising":  # scores rise for head 0 as the scales fall, and fall for head 1
+        k += np.linspace(-away, away, n)[:, None, None]
+        v *= 10.0 ** np.linspace(3.5, -3.5, n)[:, None, None]
+    elif case == "sink":  # the first token has nearly all the weight and a value near nothing
+        k[0], v[0] = away / 6, 1e-5 * v[0]
+    elif case == "zero":
+        k[0], v[0] = away / 6, 0
+    elif case == "flat":  # groups of one value, whose scale is 0
+        v[:n // 2] = v[:n // 2, :, :1]
+    elif case == "steep":  # (their bound says nothing: the result has to be finite)
+        k, v = 1e5 * k, 1e4 * v
+    return k.astype(np.float32), v.astype(np.float32), q.astype(np.float32)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hd,queries", [(32, 1), (64, 1), (128, 1), (64, 6), (128, 6)])
+@pytest.mark.parametrize("case", ["early", "late", "groups", "rising", "sink", "zero", "flat", "steep"])
+def test_scales_far_apart_cost_a_row_nothing(gpu, case, hd, queries, dtype):
+    """A value's weight keeps its bits whatever the scale of tokens that this row, or this group of 64 dims,
+    gives no weight to."""
+    rng = np.random.default_rng(hd + queries)
+    n, page = 1500, 32
+    table, pool, ks, vs = cache(rng, [n], 1, hd, page)
+    k, v, q = uneven(case, rng, n, hd)
+    for which, x, kept in ((0, k, ks), (1, v, vs)):
+        c, s, o = twin.quantise(x)
+        for i in range(n):
+            pool.put(table[0, i // page], i % page, which, c[i], s[i], o[i])
+        kept[0] = (twin.values(c, s, o), twin.magnitudes(c, s, o))
+    q = torch.from_numpy(np.broadcast_to(q, (1, queries, 2, hd)).copy()).to(dtype).cuda()
+    out = torch.empty_like(q)
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32([n]), out, 1, page)
+    check(q, out, [n], ks, vs, hd ** -0.5)
+    assert K.raw_check() is None

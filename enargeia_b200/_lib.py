@@ -111,6 +111,7 @@ SIGNATURES = {
     "enx_pages_compact": (C.c_int32, [P, P, P, P, P, P, P, P, C.POINTER(PagesDims), P, P]),
     "enx_pages_copy": (C.c_int32, [P, U32, U32, U32, P, U32, P, P, P]),
     "enx_kv4_write": (C.c_int32, [P, P, C.POINTER(C.c_int64), U32, P, P, P, P, P, P, C.POINTER(Kv4Dims), P]),
+    "enx_kv4_write_held": (C.c_int32, [P, P, C.POINTER(C.c_int64), U32, P, P, P, P, P, P, P, C.POINTER(Kv4Dims), P]),
     "enx_attn_kv4": (C.c_int32, [P, C.POINTER(C.c_int64), P, P, P, P, P, U32, U32, U32, F32, C.POINTER(Kv4Dims), P, P]),
     "enx_attn_kv4_workspace_bytes": (C.c_size_t, [U32, U32]),
     "enx_attn_packed": (C.c_int32, [P, P, P, P, C.POINTER(C.c_int64), P, U32, U32, U32, U32, U32, U32, F32, P]),

@@ -69,6 +69,7 @@ struct WriteArgs {
     long long k_token, k_head, v_token, v_head;  // strides in elements
     uint8_t* pool;
     const int32_t *table, *seqs, *positions;
+    const int32_t* lengths;  // or null: positions are taken as they are
     uint32_t tokens, rows, width, pages, page_shift, kv_heads, hd, head_shift;
     int vec;  // all rows start on 16 bytes
 };
@@ -109,7 +110,8 @@ __global__ void __launch_bounds__(256) k_kv4_write(WriteArgs a) {
                 for (int i = 0; i < 8; ++i) raw[kv][i] = src[i];
             }
         }
-        if (pos >= 0 && seq >= 0 && (uint32_t)seq < a.rows && ((uint32_t)pos >> a.page_shift) < a.width)
+        if (pos >= 0 && seq >= 0 && (uint32_t)seq < a.rows && ((uint32_t)pos >> a.page_shift) < a.width &&
+            (!a.lengths || pos < a.lengths[seq]))
             page = a.table[(size_t)seq * a.width + ((uint32_t)pos >> a.page_shift)];
     } else {
 #pragma unroll
@@ -1119,15 +1121,14 @@ cudaError_t kv4_take_error(uint32_t* code) {
 
 using namespace enx;
 
-extern "C" enx_status enx_kv4_write(const void* k, const void* v, const int64_t* strides, uint32_t tokens,
-                                    uint8_t* pool, const int32_t* table, const int32_t* seqs, const int32_t* positions,
-                                    void* k_out, void* v_out, const enx_kv4_dims* d, void* stream) {
-    ENX_TRY(check_cache(d, "enx_kv4_write"));
+static enx_status kv4_write(const std::string& w, const void* k, const void* v, const int64_t* strides, uint32_t tokens,
+                            uint8_t* pool, const int32_t* table, const int32_t* lengths, const int32_t* seqs,
+                            const int32_t* positions, void* k_out, void* v_out, const enx_kv4_dims* d, void* stream) {
+    ENX_TRY(check_cache(d, w));
     if (tokens == 0) return ENX_OK;
-    if (!k || !v || !strides || !pool || !table || !seqs || !positions)
-        return fail(ENX_ERR_INVALID, "enx_kv4_write: null pointer");
-    if (reinterpret_cast<uintptr_t>(pool) % 16) return fail(ENX_ERR_INVALID, "enx_kv4_write: the pool must be 16-byte aligned");
-    WriteArgs a{k, v, k_out, v_out, strides[0], strides[1], strides[2], strides[3], pool, table, seqs, positions, tokens,
+    if (!k || !v || !strides || !pool || !table || !seqs || !positions) return fail(ENX_ERR_INVALID, w + ": null pointer");
+    if (reinterpret_cast<uintptr_t>(pool) % 16) return fail(ENX_ERR_INVALID, w + ": the pool must be 16-byte aligned");
+    WriteArgs a{k, v, k_out, v_out, strides[0], strides[1], strides[2], strides[3], pool, table, seqs, positions, lengths, tokens,
                 d->rows, d->width, d->pages, log2_of(d->page_tokens), d->kv_heads, d->head_dim, log2_of(d->head_dim / 8), 0};
     const size_t size = d->dtype == ENX_F32 ? 4 : 2;
     uintptr_t any = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_out) |
@@ -1136,7 +1137,7 @@ extern "C" enx_status enx_kv4_write(const void* k, const void* v, const int64_t*
     a.vec = any % 16 == 0;
     const uint64_t threads = (uint64_t)tokens * d->kv_heads * (d->head_dim / 8), blocks = (threads + 255) / 256;
     const uint32_t grid = (uint32_t)blocks;
-    if (blocks * 256 > 0xffffffffull) return fail(ENX_ERR_RANGE, "enx_kv4_write: too many tokens for one call");
+    if (blocks * 256 > 0xffffffffull) return fail(ENX_ERR_RANGE, w + ": too many tokens for one call");
     if (d->dtype == ENX_F32)
         k_kv4_write<float><<<grid, 256, 0, as_stream(stream)>>>(a);
     else if (d->dtype == ENX_F16)
@@ -1145,6 +1146,20 @@ extern "C" enx_status enx_kv4_write(const void* k, const void* v, const int64_t*
         k_kv4_write<__nv_bfloat16><<<grid, 256, 0, as_stream(stream)>>>(a);
     ENX_CUDA(cudaGetLastError());
     return ENX_OK;
+}
+
+extern "C" enx_status enx_kv4_write(const void* k, const void* v, const int64_t* strides, uint32_t tokens,
+                                    uint8_t* pool, const int32_t* table, const int32_t* seqs, const int32_t* positions,
+                                    void* k_out, void* v_out, const enx_kv4_dims* d, void* stream) {
+    return kv4_write("enx_kv4_write", k, v, strides, tokens, pool, table, nullptr, seqs, positions, k_out, v_out, d, stream);
+}
+
+extern "C" enx_status enx_kv4_write_held(const void* k, const void* v, const int64_t* strides, uint32_t tokens,
+                                         uint8_t* pool, const int32_t* table, const int32_t* lengths, const int32_t* seqs,
+                                         const int32_t* positions, void* k_out, void* v_out, const enx_kv4_dims* d,
+                                         void* stream) {
+    if (tokens && !lengths) return fail(ENX_ERR_INVALID, "enx_kv4_write_held: null pointer");
+    return kv4_write("enx_kv4_write_held", k, v, strides, tokens, pool, table, lengths, seqs, positions, k_out, v_out, d, stream);
 }
 
 extern "C" size_t enx_attn_kv4_workspace_bytes(uint32_t batch, uint32_t head_dim) {

@@ -300,10 +300,11 @@ def _pool_of(pool: torch.Tensor):
     return pool.shape
 
 
-def kv4_write(k, v, pool, table, seqs, positions, page_tokens, k_out=None, v_out=None, stream=None):
+def kv4_write(k, v, pool, table, seqs, positions, page_tokens, k_out=None, v_out=None, stream=None, lengths=None):
     """Quantises k and v [tokens, kv_heads, head_dim] into the 4-bit cache: token i to position
     positions[i] of table row seqs[i] (int32; a negative position is passed over).  k_out and v_out,
-    if given, receive the values that the cache now holds."""
+    if given, receive the values that the cache now holds.  With lengths (int32 [rows]) a position at or
+    past its row's length is passed over too: nothing is written where `pages_grow` was refused."""
     shape = k.shape
     tokens, kv_heads, hd = shape
     if v.shape != shape or v.dtype is not k.dtype:
@@ -315,9 +316,10 @@ def kv4_write(k, v, pool, table, seqs, positions, page_tokens, k_out=None, v_out
     pages, nbytes = _pool_of(pool)
     k0, k1, _ = k.stride()
     v0, v1, _ = v.stride()
-    _call_on((k, v, pool, table, seqs, positions, k_out, v_out), stream, "enx_kv4_write", _rows_of(k), _rows_of(v),
-             _strides(k0, k1, v0, v1), tokens, _ptr(pool), _ints(table, r * w), _ints(seqs, tokens), _ints(positions, tokens),
-             _ptr(k_out), _ptr(v_out), _kv4_block(r, w, pages, nbytes, page_tokens, kv_heads, hd, k.dtype))
+    held = () if lengths is None else (_ints(lengths, r),)
+    _call_on((k, v, pool, table, seqs, positions, k_out, v_out, lengths), stream, "enx_kv4_write_held" if held else "enx_kv4_write",
+             _rows_of(k), _rows_of(v), _strides(k0, k1, v0, v1), tokens, _ptr(pool), _ints(table, r * w), *held, _ints(seqs, tokens),
+             _ints(positions, tokens), _ptr(k_out), _ptr(v_out), _kv4_block(r, w, pages, nbytes, page_tokens, kv_heads, hd, k.dtype))
 
 
 def attn_kv4(q, pool, table, lengths, out, kv_heads, page_tokens, seqs=None, scale=None, workspace=None, stream=None):

@@ -312,11 +312,21 @@ typedef struct {
  * group that holds a value which is not finite reads back as NaN.  Tokens with a negative position,
  * or whose row, position or page is outside the table or the pool, are passed over.  k_out and v_out
  * (contiguous, or NULL) receive the values that the cache now holds, so that a prompt's own attention
- * can see what later tokens will.  No two tokens of a call may share a slot. */
+ * can see what later tokens will.  No two tokens of a call may share a slot, and a position has to be one
+ * that the row holds: after a refused enx_pages_grow its last page may still be another row's too. */
 ENX_API enx_status enx_kv4_write(const void* k, const void* v, const int64_t* strides,
                                  uint32_t tokens, uint8_t* pool, const int32_t* table,
                                  const int32_t* seqs, const int32_t* positions, void* k_out,
                                  void* v_out, const enx_kv4_dims* dims, void* stream);
+
+/* The same, but passes over tokens at positions outside 0 .. lengths[row] - 1 (lengths int32 [rows], as
+ * enx_pages_grow leaves it), so that a step whose host does not look at the status of its grow writes
+ * nothing where that was refused. */
+ENX_API enx_status enx_kv4_write_held(const void* k, const void* v, const int64_t* strides,
+                                      uint32_t tokens, uint8_t* pool, const int32_t* table,
+                                      const int32_t* lengths, const int32_t* seqs,
+                                      const int32_t* positions, void* k_out, void* v_out,
+                                      const enx_kv4_dims* dims, void* stream);
 
 /* Attention of the `queries` newest tokens of each of `batch` sequences: sequence b is table row
  * seqs[b] (seqs NULL: row b), its cache holds lengths[row] tokens, those of the queries included, and

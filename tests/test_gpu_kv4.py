@@ -455,3 +455,75 @@ def test_scales_far_apart_cost_a_row_nothing(gpu, case, hd, queries, dtype):
     K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32([n]), out, 1, page)
     check(q, out, [n], ks, vs, hd ** -0.5)
     assert K.raw_check() is None
+
+
+def test_a_refused_grow_writes_nothing(gpu):
+    """A row cut into the middle of a page that it shares, and no page left to copy it to: the other
+    holder's tokens stay as they are, in a captured step whose host does not look at the status."""
+    rng = np.random.default_rng(18)
+    kv, hd, page = 2, 64, 16
+    table, lengths = i32(np.full((4, 4), -1)), i32([0] * 4)
+    refs, status, count, pairs = i32([0] * 4), i32([0]), i32([0, 0]), i32([[0, 0]] * 4)
+    pool = torch.zeros(1, 4, K.kv4_page_bytes(page, kv, hd), dtype=torch.uint8, device="cuda")
+    k, v = rows(rng, (32, kv, hd), F16), rows(rng, (32, kv, hd), F16)
+    K.pages_grow(table, lengths, refs, i32([0, 2]), i32([32, 16]), pairs, count, status, page)
+    K.kv4_write(k, v, pool[0], table, i32([0] * 32), i32(np.arange(32)), page, lengths=lengths)
+    K.pages_fork(table, lengths, refs, i32([0]), i32([1]), status, page)
+    K.pages_free(table, lengths, refs, i32([1]), i32([20]), status, page)
+    ko, vo = torch.full((2, kv, hd), 3.0, dtype=F16, device="cuda"), torch.full((2, kv, hd), 4.0, dtype=F16, device="cuda")
+    # row 1 wants a copy of its last page, row 3 (empty) a page: one is left
+    which, one = i32([1, 3]), i32([1, 1])
+    ps = torch.empty(K._lib.load().enx_pages_workspace_bytes(4, 4), dtype=torch.uint8, device="cuda")
+
+    def step():
+        at = lengths[which.long()]
+        K.pages_grow(table, lengths, refs, which, one, pairs, count, status, page, ps)
+        K.pages_copy(pool, pairs, count, status)
+        K.kv4_write(k[:2], v[:2], pool[0], table, which, at, page, ko, vo, lengths=lengths)
+
+    state = [x.clone() for x in (table, lengths, refs, pool)]
+    step()
+    assert status.item() == 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    graph.replay()
+    assert all(torch.equal(x, y) for x, y in zip((table, lengths, refs, pool), state))
+    assert (ko == 3).all() and (vo == 4).all()
+    # with a page given back the same graph writes both
+    K.pages_free(table, lengths, refs, i32([2]), i32([0]), status, page)
+    status.zero_()
+    graph.replay()
+    assert status.item() == 0 and lengths.tolist() == [32, 21, 0, 1]
+    want = twin.Pool(4, page, kv, hd)
+    want.bytes[:] = state[3][0].cpu().numpy()
+    t = table.tolist()
+    assert t[1][1] not in t[0] and t[3][0] not in t[0] + t[1]
+    want.bytes[t[1][1]] = want.bytes[t[0][1]]
+    for i, (page_no, slot) in enumerate(((t[1][1], 4), (t[3][0], 0))):
+        for part, x in enumerate((k, v)):
+            want.put(page_no, slot, part, *twin.quantise(x[i].float().cpu().numpy()))
+    assert (pool[0].cpu().numpy() == want.bytes).all()
+    for part, back in enumerate((ko, vo)):
+        x = (k, v)[part][:2].float().cpu().numpy()
+        assert (back.cpu().numpy() == twin.values(*twin.quantise(x)).astype(np.float16)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_lengths_bound_what_is_written(gpu, dtype):
+    """Positions at and past the row's length, of rows of length zero and below, are passed over."""
+    rng = np.random.default_rng(19)
+    kv, hd, page = 1, 32, 16
+    table, lengths = i32([[0, 1], [2, 3], [4, 5]]), i32([17, 0, -4])
+    seqs, positions = i32([0, 0, 0, 1, 2, 0, 3, -1]), i32([16, 17, 31, 0, 0, 0, 0, 0])
+    k, v = rows(rng, (8, kv, hd), dtype), rows(rng, (8, kv, hd), dtype)
+    pool = torch.zeros(6, K.kv4_page_bytes(page, kv, hd), dtype=torch.uint8, device="cuda")
+    K.kv4_write(k, v, pool, table, seqs, positions, page, lengths=lengths)
+    want = twin.Pool(6, page, kv, hd)
+    for i, (at, slot) in ((0, (1, 0)), (5, (0, 0))):
+        for part, x in enumerate((k, v)):
+            want.put(at, slot, part, *twin.quantise(x[i].float().cpu().numpy()))
+    assert (pool.cpu().numpy() == want.bytes).all()
+    for bad in (i32([1, 1]), lengths.long(), lengths.cpu()):
+        with pytest.raises(ValueError):
+            K.kv4_write(k, v, pool, table, seqs, positions, page, lengths=bad)

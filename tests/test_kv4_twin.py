@@ -62,3 +62,16 @@ def test_entry_points_refuse(lib):
     assert attn(heads=3) == 1 and attn(heads=0) == 1 and attn(scale=0.0) == 1 and attn(scale=float("nan")) == 1
     assert attn(batch=5) == 3 and attn(queries=1 << 17) == 3
     assert lib.enx_attn_kv4_workspace_bytes(256, 64) < 64 << 20
+
+
+def test_the_bounded_writer_refuses(lib):
+    from enargeia_b200._lib import Kv4Dims
+
+    p, st = C.c_void_p(256), (C.c_int64 * 4)(64, 64, 64, 64)
+
+    def write(dims=(4, 4, 8, 16, 2, 64, 0, 0), k=p, lengths=p, tokens=1):
+        return lib.enx_kv4_write_held(k, p, st, tokens, p, p, lengths, p, p, None, None, C.byref(Kv4Dims(*dims)), None)
+
+    assert write(tokens=0, lengths=None) == 0
+    assert write(lengths=None) == 1 and write(k=None) == 1 and write((4, 4, 8, 24, 2, 64, 0, 0)) == 1
+    assert b"enx_kv4_write_held" in lib.enx_last_error()

@@ -13,6 +13,7 @@
 // traffic: 2 * bytes moved.
 
 #include "enx_internal.cuh"
+#include "pages_want.h"
 
 namespace enx {
 
@@ -222,8 +223,9 @@ __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const in
         }
     }
     __syncthreads();
-    // (copies << 32 | pages) wanted by the rows before each one
-    for (uint32_t i0 = 0; i0 < n; i0 += kPgThreads) {
+    // pages and copies wanted by the rows before each one; more pages than there are end the call
+    bool enough = true;
+    for (uint32_t i0 = 0; i0 < n && enough; i0 += kPgThreads) {
         const uint32_t i = i0 + tid;
         unsigned long long mine = 0;
         if (i < n) {
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const in
             const bool copy = p >= 0 && !(__ldcg(&writers[p]) == a.refs[p] && __ldcg(&first[p]) == (int32_t)i);
             const uint32_t fresh = pages_of(lens[i] + (uint32_t)add[i], pt) - pages_of(lens[i], pt);
             if (fresh > kPgFew) s_many = 1;
-            mine = ((unsigned long long)copy << 32) + fresh + copy;
+            mine = want_of(copy, fresh, a.pages);
         }
         unsigned long long incl = mine;
 #pragma unroll
@@ -247,11 +249,12 @@ __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const in
         __syncthreads();
         if (tid == kPgThreads - 1) s_run = before + incl;
         __syncthreads();
+        enough = want_pages(s_run) <= a.pages;
     }
-    const uint32_t total = (uint32_t)s_run, copies = (uint32_t)(s_run >> 32);
+    const uint32_t total = enough ? (uint32_t)want_pages(s_run) : 0, copies = want_copies(s_run);
     // the lowest `total` free pages (a page that loses a holder to a copy keeps another one)
     uint32_t have = 0;
-    for (uint32_t base = 0; base < a.pages && have < total; base += kPgThreads * kPgRun) {
+    for (uint32_t base = 0; enough && base < a.pages && have < total; base += kPgThreads * kPgRun) {
         uint32_t flags = 0;
 #pragma unroll
         for (uint32_t j = 0; j < kPgRun; ++j) {
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const in
         }
         have += got;
     }
-    if (have < total) {  // not enough: nothing has changed
+    if (!enough || have < total) {  // not enough: nothing has changed
         if (tid == 0) atomicOr(a.status, kPgNoneFree);
         return;
     }
@@ -281,16 +284,16 @@ __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const in
         const int32_t row = list[i];
         const uint32_t old = lens[i], held = pages_of(old, pt);
         const unsigned long long at = wanted[i], next = i + 1 < n ? wanted[i + 1] : s_run;
-        const uint32_t at_page = (uint32_t)at, copy = (uint32_t)(next >> 32) - (uint32_t)(at >> 32);
-        const uint32_t fresh = (uint32_t)next - at_page - copy;
+        const uint32_t at_page = (uint32_t)want_pages(at), at_copy = want_copies(at), copy = want_copies(next) - at_copy;
+        const uint32_t fresh = (uint32_t)want_pages(next) - at_page - copy;
         int32_t* entries = a.table + (size_t)row * a.width;
         if (copy) {
             const int32_t from = last[i], to = found[at_page];
             entries[old / pt] = to;
             a.refs[to] = 1;
             atomicSub(&a.refs[from], 1);
-            pairs[2 * (at >> 32)] = from;
-            pairs[2 * (at >> 32) + 1] = to;
+            pairs[2 * at_copy] = from;
+            pairs[2 * at_copy + 1] = to;
         }
         if (fresh <= kPgFew)
             for (uint32_t k = 0; k < fresh; ++k) take(entries, held, at_page + copy, k);
@@ -299,8 +302,8 @@ __global__ void __launch_bounds__(kPgThreads) k_pages_grow(PagesArgs a, const in
     if (s_many)
         for (uint32_t i = warp; i < n; i += kPgThreads / 32) {
             const unsigned long long at = wanted[i], next = i + 1 < n ? wanted[i + 1] : s_run;
-            const uint32_t at_page = (uint32_t)at, copy = (uint32_t)(next >> 32) - (uint32_t)(at >> 32);
-            const uint32_t fresh = (uint32_t)next - at_page - copy;
+            const uint32_t at_page = (uint32_t)want_pages(at), copy = want_copies(next) - want_copies(at);
+            const uint32_t fresh = (uint32_t)want_pages(next) - at_page - copy;
             if (fresh > kPgFew)
                 for (uint32_t k = lane; k < fresh; k += 32)
                     take(a.table + (size_t)list[i] * a.width, pages_of(lens[i], pt), at_page + copy, k);

@@ -224,3 +224,23 @@ def test_refused_arguments(gpu):
         K.pages_grow(t, l, r, l, l, i32([[0, 0]]), i32([0, 0]), st, 16, torch.empty(4, dtype=torch.uint8, device="cuda"))
     with pytest.raises(EnxError):
         K.pages_copy(torch.zeros(1, 2, 24, dtype=torch.uint8, device="cuda"), i32([[0, 1]]), i32([1]), st)
+
+
+def test_more_pages_wanted_than_32_bits_hold(gpu):
+    """The largest table: 262144 rows of 16384 pages that all want to be filled, 2^32 pages, which a 32-bit
+    sum takes for none.  The call is refused and changes nothing."""
+    rows, width, pages = 1 << 18, 1 << 14, 64
+    table = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")  # 17 GB
+    lengths, refs, status = i32([0] * rows), i32([0] * pages), i32([0])
+    every, add = torch.arange(rows, dtype=torch.int32, device="cuda"), torch.full((rows,), width, dtype=torch.int32, device="cuda")
+    pairs, count = torch.full((rows, 2), -7, dtype=torch.int32, device="cuda"), i32([-7, -7])
+    K.pages_grow(table, lengths, refs, every, add, pairs, count, status, 1)
+    assert status.item() == NONE_FREE and count.tolist() == [0, 0]
+    assert not lengths.any() and not refs.any() and bool((pairs == -7).all())
+    assert all(bool((table[i:i + 4096] == -1).all()) for i in range(0, rows, 4096))
+    # a few rows in its last corner, as far behind 2^32 bytes as a table goes
+    some = [rows - 1, 0, rows - 2]
+    K.pages_grow(table, lengths, refs, i32(some), i32([40, 3, 21]), pairs, count, status, 1)
+    assert status.item() == NONE_FREE and count.tolist() == [0, 64]
+    assert table[-1, :41].tolist() == [*range(40), -1] and table[0, :4].tolist() == [40, 41, 42, -1]
+    assert table[-2, :22].tolist() == [*range(43, 64), -1] and refs.tolist() == [1] * 64

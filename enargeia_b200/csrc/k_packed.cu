@@ -61,6 +61,7 @@ constexpr uint32_t kPkRows = 128;           // rows of a tile, keys of a tile
 constexpr uint32_t kPkThreads = 512;
 constexpr uint32_t kPkItems = 4;             // items between the warp that finds them and the others
 constexpr uint32_t kPkClean = 4;             // barriers of partly seen V tiles: more than a ring holds
+constexpr uint32_t kPkFoul = 2;              // flags of items whose partly seen V tiles were not all finite (below)
 constexpr uint32_t kPkTileBytes = 128 * 128;  // 128 rows of 64 16-bit elements
 constexpr int kPkRegs = 128, kPkRegsSoftmax = 192, kPkRegsOut = 88, kPkRegsRest = 40;
 static_assert(2 * kPkRegsSoftmax + kPkRegsOut + kPkRegsRest <= 4 * kPkRegs, "the warpgroups' registers come out of the launch's");
@@ -311,12 +312,15 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     __shared__ float s_inv[2][128];
     __shared__ uint32_t tmem_base;
     __shared__ volatile int s_fail;
-    __shared__ uint32_t s_foul;  // 1 + the last item in whose partly seen V tiles an element was not finite
+    // 1 + the last item of its parity in whose partly seen V tiles an element was not finite.  Two, as an output
+    // warp may clean the next item's tiles while another has yet to look at this one's flag; before the flag's next
+    // use, two items on, every thread has arrived on a barrier of the item between, behind its look.
+    __shared__ uint32_t s_foul[kPkFoul];
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 32) {
         s_fail = 0;
-        s_foul = 0;
+        for (uint32_t i = 0; i < kPkFoul; ++i) s_foul[i] = 0;
         auto init = [](uint64_t* bar, uint32_t count) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(bar)), "r"(count));
         };
@@ -550,15 +554,15 @@ __global__ void __launch_bounds__(kPkThreads, 1)
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(v + i * 16), "r"(x[0]), "r"(x[1]), "r"(x[2]),
                                      "r"(x[3])
                                      : "memory");
-                        s_foul = k + 1;
+                        s_foul[k % kPkFoul] = k + 1;
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&v_clean[clean % kPkClean]);
-                ok = ok && wait(&v_clean[clean % kPkClean], clean / kPkClean);  // every thread's part: s_foul is settled
+                ok = ok && wait(&v_clean[clean % kPkClean], clean / kPkClean);  // every thread's part: the flag is settled
             }
             ok = __all_sync(0xffffffffu, ok);
-            const bool foul = ok && *(volatile uint32_t*)&s_foul == k + 1;
+            const bool foul = ok && *(volatile uint32_t*)&s_foul[k % kPkFoul] == k + 1;
             ring += 2 * n;
 #pragma unroll
             for (uint32_t w = 0; w < 2; ++w) {

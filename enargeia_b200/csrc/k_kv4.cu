@@ -180,6 +180,11 @@ __global__ void __launch_bounds__(256) k_kv4_write(WriteArgs a) {
         T* back = static_cast<T*>(kv ? a.v_out : a.k_out);
         if (back) {
             alignas(16) T tmp[8];
+            // 15 steps of a scale that was rounded up may pass f16's largest number: it saturates here as there
+            if (std::is_same<T, __half>::value && fmaf(s, 15.f, m) > 65504.f) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) val[i] = fminf(val[i], 65504.f);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) tmp[i] = from_f<T>(val[i]);
             if (a.vec) {

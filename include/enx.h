@@ -311,7 +311,8 @@ typedef struct {
  * (x - offset) / scale to the nearest whole number (ties to even), 0 to 15; f16 saturates.  A
  * group that holds a value which is not finite reads back as NaN.  Tokens with a negative position,
  * or whose row, position or page is outside the table or the pool, are passed over.  k_out and v_out
- * (contiguous, or NULL) receive the values that the cache now holds, so that a prompt's own attention
+ * (contiguous, or NULL) receive the values that the cache now holds, rounded to dtype (f16: 65504
+ * where a code stands for more), so that a prompt's own attention
  * can see what later tokens will.  No two tokens of a call may share a slot, and a position has to be one
  * that the row holds: after a refused enx_pages_grow its last page may still be another row's too. */
 ENX_API enx_status enx_kv4_write(const void* k, const void* v, const int64_t* strides,

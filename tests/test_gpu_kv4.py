@@ -527,3 +527,21 @@ def test_lengths_bound_what_is_written(gpu, dtype):
     for bad in (i32([1, 1]), lengths.long(), lengths.cpu()):
         with pytest.raises(ValueError):
             K.kv4_write(k, v, pool, table, seqs, positions, page, lengths=bad)
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+def test_values_at_the_end_of_f16_stay_finite(gpu, hd):
+    """15 steps of a rounded scale may pass 65504, which f16 rows read back as 65504."""
+    k = torch.linspace(0, 65504, hd, device="cuda").half().repeat(3, 2, 1)
+    v = -k
+    k[1, 0] -= 30000
+    k[2], v[2] = torch.linspace(-65504, 65504, hd, device="cuda").half(), 1.0
+    pool = torch.zeros(1, K.kv4_page_bytes(16, 2, hd), dtype=torch.uint8, device="cuda")
+    ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+    K.kv4_write(k, v, pool, i32([[0]]), i32([0, 0, 0]), i32([0, 1, 2]), 16, ko, vo)
+    past = 0
+    for x, back in ((k, ko), (v, vo)):
+        held = twin.values(*twin.quantise(x.float().cpu().numpy()))
+        past += int((held > 65504).sum())
+        assert (back.cpu().numpy() == np.minimum(held, 65504.0).astype(np.float16)).all()
+    assert past > 0

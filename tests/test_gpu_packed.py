@@ -333,3 +333,25 @@ def test_a_weight_that_underflows_is_zero(gpu, hd, dtype, big):
     v[:4] = big
     K.attn_packed(q, k, v, loud, ends)
     assert torch.equal(quiet[4:], loud[4:]) and (loud[0] == v[0]).all()
+
+
+def test_waits_that_run_out_raise_the_error(gpu):
+    """An item of 512 key tiles takes most of a millisecond, and its output waits for all of it: one poll is
+    not enough.  The status says so, and the next call is whole again."""
+    q, k, v, ends = make([1 << 16], 1, 1, 64, BF16, 18)
+    out = torch.empty_like(q)
+    K.raw_check()
+    try:
+        K.set_wait_limit(1)
+        K.attn_packed(q, k, v, out, ends)
+        with pytest.raises(EnxError) as e:
+            K.raw_check()
+        assert e.value.status == 5 and "enx_attn_packed" in str(e.value)
+        K.raw_check()  # read and cleared
+    finally:
+        K.set_wait_limit(0)
+    q, k, v, ends = make([700, 90], 1, 1, 64, BF16, 19)
+    out = torch.empty_like(q)
+    K.attn_packed(q, k, v, out, ends)
+    K.raw_check()
+    check(out, q, k, v, ends)

@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ?
     uint32_t qf[NT][G * KW * 2][2], ql[SPLIT ? NT : 1][SPLIT ? G * KW * 2 : 1][2];
     float kfac[NT][2], qsum[NT][2][G];
     int32_t last[NT][2];  // the last token a column sees
-    // m: a row's reference, lu: log2 of the unit of its weights in each group, whole numbers both
+    // m: a row's reference, lu: log2 of the unit of its weights in each group, a whole number
     float m[NT][2], l[NT][2], o[NT][MT][4], om[NT][2][G], lu[NT][2][G];
 
     uint32_t begun = 0;  // the unit of the run with which the present head began
@@ -762,8 +762,10 @@ __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ?
                         over = over || tops[n][j] - m[n][j] > fminf(8.f, room[gr] - lu[n][j][gr]);
                 }
             if (__any_sync(0xffffffffu, over)) {
-                // New references: the rows' maxima.  New units: the largest weight so far comes to 16 to 32 (what the
-                // unit says of the earlier ones, less what the reference's move takes off, or this tile's).
+                // New references: the maxima of the rows that are past theirs (themselves, unrounded: the weight of a
+                // token that has it all is then 1, and its scale loses nothing in f16).  New units: the largest weight
+                // so far comes to 16 to 32 (what the unit says of the earlier ones, less what the reference's move
+                // takes off, or this tile's).  A move of 8 and more costs that estimate less than 1 in rounding.
                 float lv[2][2][G];
 #pragma unroll
                 for (int p = 0; p < 2; ++p)
@@ -780,7 +782,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ?
                         float top = tops[n][j], wide[G];
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        top = fmaxf(floorf(top), m[n][j]);
+                        top = top - m[n][j] > 8.f ? top : m[n][j];
                         const float moved = top - m[n][j], fm = ex2(-moved);
                         m[n][j] = top;
                         l[n][j] *= fm;
@@ -792,7 +794,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ?
                                 wide[gr] = fmaxf(wide[gr], fmaxf(sc[p][n][j] - top + lv[p][0][gr], sc[p][n][2 + j] - top + lv[p][1][gr]));
 #pragma unroll
                             for (int x = 4; x < 32; x <<= 1) wide[gr] = fmaxf(wide[gr], __shfl_xor_sync(0xffffffffu, wide[gr], x));
-                            const float unit = 4.f - fmaxf(floorf(wide[gr]), 4.f - lu[n][j][gr] - moved);
+                            const float unit = 4.f - floorf(fmaxf(wide[gr], 4.f - lu[n][j][gr] - moved));
                             f[gr][j] = fm * pow2_whole(unit - lu[n][j][gr]);
                             lu[n][j][gr] = unit;
                             om[n][j][gr] *= fm;

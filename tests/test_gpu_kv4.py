@@ -545,3 +545,29 @@ def test_values_at_the_end_of_f16_stay_finite(gpu, hd):
         past += int((held > 65504).sum())
         assert (back.cpu().numpy() == np.minimum(held, 65504.0).astype(np.float16)).all()
     assert past > 0
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_a_token_with_all_the_weight_comes_back_rounded_once(gpu, hd, dtype):
+    """Its weight is 1, and scale, code and offset are exact: what is left of the bound is the f32 sum of the
+    two terms (2^-22 of their sizes: f32 rows split them at code 8) and the output's own half step."""
+    rng = np.random.default_rng(hd)
+    lengths = [1] * 40 + [70] * 10
+    table, pool, ks, vs = cache(rng, lengths, 1, hd, 16)
+    q = np.abs(rng.standard_normal((50, 1, 4, hd))).astype(np.float32) + 0.2
+    for r in range(40, 50):  # one token far above the others, anywhere
+        at = int(rng.integers(70))
+        c, s, o = twin.quantise(np.full((1, hd), 60 * hd ** -0.5, np.float32))
+        pool.put(table[r, at // 16], at % 16, 0, c, s, o)
+        c, s, o = twin.quantise((rng.standard_normal((1, hd)) * 3).astype(np.float32))
+        pool.put(table[r, at // 16], at % 16, 1, c, s, o)
+        vs[r] = (twin.values(c, s, o)[None], twin.magnitudes(c, s, o)[None])
+    q = torch.from_numpy(q).to(dtype).cuda()
+    out = torch.empty_like(q)
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32(lengths), out, 1, 16, scale=1.0)
+    half = torch.finfo(dtype).eps / 2
+    for r in range(50):
+        value, size = vs[r][0][0, 0], vs[r][1][0, 0]
+        off = np.abs(out[r, 0].double().cpu().numpy() - value) - (half * np.abs(value) * (1 + 2.0 ** -11) + 2.0 ** -22 * size)
+        assert (off <= 0).all(), (r, float(off.max()))

@@ -378,8 +378,10 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 // its value, and cuts off what falls below, so f32 rows take the codes as normal numbers, c - 8 (one
 // more instruction for two elements, and less to cancel between scale and offset), and sum 32 tokens
 // by themselves before the long sum in f32 (4e-6 off without either, 1e-7 with both).  16-bit rows
-// need one operand (an f16 or bf16 q fits f16 after a power of two is taken out; w is rounded to f16,
-// half a step 2^-11, before a sum that is rounded to 16 bits anyway).
+// need one operand for q (f16 or bf16, it fits f16 after a power of two is taken out).  bf16 rows need one for
+// w too: its rounding to f16, half a step 2^-11, is an eighth of the output's half step 2^-8 even where scale *
+// code cancels against the offset.  In f16 rows that rounding would be as large as the output's own (few tokens
+// with weight: 1.7 times the error of f32 sums), so they take w as two.
 //
 // Bound: 4.5 bits a value leave two to three instructions a value at full HBM rate, and the loop needs about
 // three (256 sequences up to 2048 tokens, 14/2 heads of 64, f32: 30 us, 1.3 TB/s, a quarter of it at the heads'
@@ -396,6 +398,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ?
     constexpr uint32_t kRow = HD / 2, kTokenBytes = HD + 8 * G;
     constexpr uint32_t kStageBytes = kKvChunk * kTokenBytes;
     constexpr uint32_t kCols = 8 * NT;
+    constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;  // w as two f16 each
     // the operands' units: subnormal codes are 2^-24, and every second one is 16-fold
     constexpr int kExp = SPLIT ? 0 : 24;
     constexpr float kOdd = SPLIT ? 1.f : 0.0625f, kUp = SPLIT ? 1.f : 0x1p24f;
@@ -836,7 +839,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ?
                         const uint32_t h0 = pack_h2(x[0], x[1]), h1 = pack_h2(x[2], x[3]);
                         wb[p][n][0] = transpose8x8(h0);
                         wb[p][n][1] = transpose8x8(h1);
-                        if (SPLIT) {
+                        if (kTwo) {
                             const float2 r0 = unpack_h2(h0), r1 = unpack_h2(h1);
                             wl[p][n][0] = transpose8x8(pack_h2(x[0] - r0.x, x[1] - r0.y));
                             wl[p][n][1] = transpose8x8(pack_h2(x[2] - r1.x, x[3] - r1.y));
@@ -884,6 +887,10 @@ __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ?
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) o[n][d][e] += add[e];
                             } else {
+                                if (kTwo) {
+#pragma unroll
+                                    for (int p = 0; p < 2; ++p) mma16816(o[n][d], af[p], wl[p][n][0], wl[p][n][1]);
+                                }
 #pragma unroll
                                 for (int p = 0; p < 2; ++p) mma16816(o[n][d], af[p], wb[p][n][0], wb[p][n][1]);
                             }

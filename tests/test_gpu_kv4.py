@@ -571,3 +571,20 @@ def test_a_token_with_all_the_weight_comes_back_rounded_once(gpu, hd, dtype):
         value, size = vs[r][0][0, 0], vs[r][1][0, 0]
         off = np.abs(out[r, 0].double().cpu().numpy() - value) - (half * np.abs(value) * (1 + 2.0 ** -11) + 2.0 ** -22 * size)
         assert (off <= 0).all(), (r, float(off.max()))
+
+
+@pytest.mark.parametrize("heads,kv,hd,queries", [(14, 2, 64, 1), (4, 2, 32, 1), (16, 2, 128, 1), (14, 2, 64, 3), (16, 2, 128, 4)])
+def test_f16_rows_lose_no_more_than_the_outputs_rounding(gpu, heads, kv, hd, queries):
+    """f16 rows are held to the bound of f32 rows (`weight` 0: no further rounding of the weights) and half a step
+    of the output.  Small scores, so that the bound's share of them is small too."""
+    rng = np.random.default_rng(hd + queries)
+    lengths = [4, 5, 7, 9, 17, 33, 60, 64, 65, 130, 300]
+    table, pool, ks, vs = cache(rng, lengths, kv, hd, 32)
+    q = torch.from_numpy(0.05 * rng.standard_normal((len(lengths), queries, heads, hd)).astype(np.float32)).half().cuda()
+    out = torch.empty_like(q)
+    K.attn_kv4(q, torch.from_numpy(pool.bytes).cuda(), i32(table), i32(lengths), out, kv, 32)
+    half = torch.finfo(F16).eps / 2
+    for b in range(len(lengths)):
+        want, bound = twin.attention(q[b].double().cpu().numpy(), ks[b][0], vs[b][0], hd ** -0.5, queries, ks[b][1], vs[b][1])
+        off = np.abs(out[b].double().cpu().numpy() - want) - (bound * (1 + half) + half * np.abs(want) + 2.0 ** -25)
+        assert (off <= 0).all(), (b, float(off.max()))

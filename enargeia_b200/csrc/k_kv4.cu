@@ -384,10 +384,13 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 // with weight: 1.7 times the error of f32 sums), so they take w as two.
 //
 // Bound: 4.5 bits a value leave two to three instructions a value at full HBM rate, and the loop needs about
-// three (256 sequences up to 2048 tokens, 14/2 heads of 64, f32: 30 us, 1.3 TB/s, a quarter of it at the heads'
-// ends; 32 us without their place in the split; four up to 131072, 32/8 heads of 128, bf16: 105 us, 4.2 TB/s; ALU pipe 40 to 50 % busy, issue 55 to 60 %);
-// tcgen05 would want the codes widened into shared memory first, which costs more than
-// the products do on mma.sync at 8 rows.
+// three.  No pipe is at its end, though: 45 to 58 % of the issue slots are used (ALU pipe 35 to 51 %, tensor 17 to
+// 24 %), and most of a warp's other cycles go to the fixed latencies of the chain scores - vote - exponential -
+// pack - movmatrix - product, which three warps a scheduler do not hide.  256 sequences up to 2048 tokens, 14/2
+// heads of 64, f32: 30 us, 1.3 TB/s, a quarter of it at the heads' ends (32 us without their place in the
+// split); four up to 131072, 32/8 heads of 128, bf16: 107 us, 4.0 TB/s; 24 up to 5000, 4 queries, f16: 23 us.
+// tcgen05 would want the codes widened into shared memory first, which costs more than the products do on
+// mma.sync at 8 rows.
 // Three CTAs an SM where their 168 registers suffice: left to itself the compiler takes 182 to 189 and two.
 template <typename T, int HD, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ? 3 : 2) k_kv4_attn(AttnArgs a) {
@@ -437,6 +440,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, HD * NT <= (SPLIT ? 64 : 128) ?
     }
     s_before[tid] = before;
     const uint32_t runs = gridDim.x * kKvWarps;
+    // A head is cut into 257 pieces at most, by the longest that the table can hold: so a table much wider than its
+    // sequences makes long runs for few warps (the 256 sequences above: 30 us with 2048 tokens a row, 38 us with
+    // 131072, 117 us with 2^20).
     const uint32_t per = max(max(kKvMinRun, (a.most_chunks + 255) / 256), (total + runs - 1) / runs);
     if (blockIdx.x == 0) {  // what the join needs to find the pieces
         uint32_t at = before;

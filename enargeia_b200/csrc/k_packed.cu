@@ -20,8 +20,9 @@
 // are 1024 clocks, their products 512 at hd 64 and 1024 at hd 128; so at hd 128 some exponentials are
 // taken on the FMA pipe instead (2^x = 2^n 2^f, a cubic in f).
 //
-// Measured: 16 prompts up to 2048 tokens, 14/2 heads of 64, 114 us (419 TFLOP/s); three up to 12001, 32/8 heads of
-// 128, 1455 us (1030 TFLOP/s); one of 16384, 16/2 heads, 725 and 1213 TFLOP/s at hd 64 and 128.
+// Measured: 16 prompts up to 2048 tokens, 14/2 heads of 64, 115 us (414 TFLOP/s); three up to 12001, 32/8 heads of
+// 128, 1440 us (1040 TFLOP/s) in passes one behind another, where the card is at its 1000 W and runs at 1640 MHz,
+// and 1274 us (1174 TFLOP/s) alone; one of 16384, 16/2 heads, alone, 741 and 1239 TFLOP/s at hd 64 and 128.
 //
 // One CTA per SM works through items, the next one's loads and first products under the present one's
 // last weights and output.  Items are in descending order of their key tiles, over all prompts and

@@ -87,7 +87,8 @@ ENX_API enx_status enx_matmul_q4(const float* x, const uint32_t* packed, const f
 ENX_API enx_status enx_raw_check(void);
 
 /* How many polls a bounded device-side wait (grid barrier, readiness counter, ring or pipeline
- * mbarrier of the persistent decode kernel and of the tensor-core GEMM) makes on `device` before
+ * mbarrier of the persistent decode kernel, of the tensor-core GEMM, of enx_attn_kv4 and of
+ * enx_attn_packed) makes on `device` before
  * it gives up and the call reports ENX_ERR_TIMEOUT; 0 restores the default (2^24 polls, well
  * under a minute).  A waiting CTA that gives up still waits, with the default limit, for the
  * copies and MMAs it issued before it exits.  Applies to launches made after the call (CUDA graphs
@@ -235,7 +236,8 @@ ENX_API enx_status enx_add(const float* a, const float* b, float* out, uint32_t 
  * a number is negative or a row would outgrow its table, it raises ENX_PAGES_BAD_LIST in *status
  * (device int32, bits are added, the caller clears them), and where pages run out
  * ENX_PAGES_NONE_FREE, and changes nothing.  A page number outside the pool raises
- * ENX_PAGES_BAD_PAGE and is passed over.  ENX_ERR_RANGE above 262144 rows, 2^28 pages or 2^31 - 1
+ * ENX_PAGES_BAD_PAGE and is passed over (but enx_pages_grow, which has to look at a partly filled last
+ * page, refuses such a row with ENX_PAGES_BAD_LIST).  ENX_ERR_RANGE above 262144 rows, 2^28 pages or 2^31 - 1
  * tokens a row. */
 typedef struct {
     uint32_t rows, width, pages, page_tokens;
@@ -312,9 +314,9 @@ typedef struct {
  * group that holds a value which is not finite reads back as NaN.  Tokens with a negative position,
  * or whose row, position or page is outside the table or the pool, are passed over.  k_out and v_out
  * (contiguous, or NULL) receive the values that the cache now holds, rounded to dtype (f16: 65504
- * where a code stands for more), so that a prompt's own attention
- * can see what later tokens will.  No two tokens of a call may share a slot, and a position has to be one
- * that the row holds: after a refused enx_pages_grow its last page may still be another row's too. */
+ * where a code stands for more), so that a prompt's own attention can see what later tokens will.  No
+ * two tokens of a call may share a slot, and a position has to be one that the row holds: after a
+ * refused enx_pages_grow its last page may still be another row's too. */
 ENX_API enx_status enx_kv4_write(const void* k, const void* v, const int64_t* strides,
                                  uint32_t tokens, uint8_t* pool, const int32_t* table,
                                  const int32_t* seqs, const int32_t* positions, void* k_out,
@@ -334,8 +336,10 @@ ENX_API enx_status enx_kv4_write_held(const void* k, const void* v, const int64_
  * query j sees tokens 0 .. lengths[row] - queries + j.  q is [batch][queries][heads][head_dim] with
  * strides[0..2] of its first three axes in elements, out the same, contiguous and 16-byte aligned;
  * softmax of scale * q.k.  Query rows that see nothing are 0; where seqs[b] is no table row, out is left as it was (a
- * padded batch); a page number outside the pool makes its sequence's rows NaN.  Softmax and sums in
- * f32.  workspace: enx_attn_kv4_workspace_bytes, 16-byte aligned, one for each call that may overlap
+ * padded batch); a page number outside the pool makes its sequence's rows NaN.  Scores, softmax and
+ * sums in f32; for the product with V's codes the weights go in as two f16 each (2^-22), with bf16 rows as
+ * one (2^-11).  |q| up to 2^80.  A sequence's result may differ in its last bits (within the f32 sums'
+ * rounding) with the batch that it is in, as the split of the work does.  workspace: enx_attn_kv4_workspace_bytes, 16-byte aligned, one for each call that may overlap
  * on the GPU.  enx_raw_check reports a bounded wait that gave up. */
 ENX_API enx_status enx_attn_kv4(const void* q, const int64_t* strides, const uint8_t* pool,
                                 const int32_t* table, const int32_t* lengths, const int32_t* seqs,
@@ -352,7 +356,9 @@ ENX_API size_t enx_attn_kv4_workspace_bytes(uint32_t batch, uint32_t head_dim);
  * ENX_F16 or ENX_BF16; head_dim a multiple of 8, at most 128; at most 2^24 tokens and 65536 prompts.
  * Rows of no prompt are left as they were, and no row depends on one it does not attend, whatever
  * that holds.  Scores, softmax and sums in f32, weights rounded to the dtype for their product with
- * v.  No workspace.  enx_raw_check reports a bounded wait that gave up. */
+ * v; with heads above 64 one weight in eight is good to 7.5e-5 before that.  Each CTA goes through the
+ * offsets once or more for every 256 queries and head of its share: meant for up to a few thousand
+ * prompts a call.  No workspace.  enx_raw_check reports a bounded wait that gave up. */
 ENX_API enx_status enx_attn_packed(const void* q, const void* k, const void* v, void* out,
                                    const int64_t* strides, const int32_t* offsets, uint32_t seqs,
                                    uint32_t tokens, uint32_t heads, uint32_t kv_heads,

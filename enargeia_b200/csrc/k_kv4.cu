@@ -368,8 +368,8 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 //   tiles need no maximum across lanes (one vote); p stays below 2^8.
 //   O^T [dim][row] += V codes^T (A) * w (B), w = p * scale, which one movmatrix per 8x8 turns from
 //   the accumulator's layout into the operand's.  p * offset is summed apart, in f32 FMAs.
-//   w goes in as f16 in units of a power of two of the row's and the group's own, in which the largest w
-//   met so far is 16 to 32: a token with a large scale that this row gives no weight to, or the other
+//   w goes in as f16 in units of a power of two of the row's and the group's own, chosen so that the largest
+//   w met so far is 16 to 32, and again before one would pass f16's range: a token with a large scale that this row gives no weight to, or the other
 //   group's scales, must not take the bits of those that count.  The vote that guards m guards them too.  (A
 //   token whose V is nothing but zeros counts as one of scale 2^-25; beside it what lies 2^-50 below is lost.)
 //
@@ -379,9 +379,9 @@ __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
 // more instruction for two elements, and less to cancel between scale and offset), and sum 32 tokens
 // by themselves before the long sum in f32 (4e-6 off without either, 1e-7 with both).  16-bit rows
 // need one operand for q (f16 or bf16, it fits f16 after a power of two is taken out).  bf16 rows need one for
-// w too: its rounding to f16, half a step 2^-11, is an eighth of the output's half step 2^-8 even where scale *
-// code cancels against the offset.  In f16 rows that rounding would be as large as the output's own (few tokens
-// with weight: 1.7 times the error of f32 sums), so they take w as two.
+// w too: its rounding to f16, half a step 2^-11, is an eighth of the output's half step 2^-8 (at most 1.02
+// times the error of f32 sums, with few tokens, whose scale * code cancels against the offset).  In f16 rows it
+// would be as large as the output's own (1.7 times), so they take w as two.
 //
 // Bound: 4.5 bits a value leave two to three instructions a value at full HBM rate, and the loop needs about
 // three.  No pipe is at its end, though: 45 to 58 % of the issue slots are used (ALU pipe 35 to 51 %, tensor 17 to
